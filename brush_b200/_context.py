@@ -77,6 +77,13 @@ def context(device: torch.device | int | None = None) -> Context:
     return ctx
 
 
+def feature_context(device: torch.device) -> tuple[Context, int]:
+    """(context, current stream) for the operators that take their stream as an argument; the
+    stream the context is bound to stays as it is."""
+    ctx = _CTX.get(device.index)
+    return ctx if ctx is not None else context(device), torch.cuda.current_stream(device).cuda_stream
+
+
 class _DeviceArray:
     """Minimal ``__cuda_array_interface__`` exporter for a raw device pointer."""
 

@@ -34,6 +34,8 @@ STATUS_NAMES = {
     8: "BSX_ERR_FORMAT",
 }
 
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+ACT_NONE, ACT_SILU, ACT_GELU_TANH = 0, 1, 2
 RENDER_DEFAULT, RENDER_MIP = 0, 1
 PASS_FORWARD, PASS_BACKWARD, PASS_BACKWARD_SMOOTH_CUTOFF = 0, 1, 2
 
@@ -244,6 +246,26 @@ class RefineStats(C.Structure):
                                                  "num_pruned", "num_pruned_non_finite", "total_splats")]
 
 
+class DropoutCfg(C.Structure):
+    _fields_ = [
+        ("p", C.c_double),
+        ("seed", C.c_uint64),
+        ("share", C.c_uint64),
+        ("d_step", C.c_void_p),
+        ("step", C.c_uint32),
+    ]
+
+
+class GroupNormCfg(C.Structure):
+    _fields_ = [
+        ("groups", C.c_uint32),
+        ("eps", C.c_float),
+        ("activation", C.c_int32),
+        ("param_dtype", C.c_int32),
+        ("dropout", C.POINTER(DropoutCfg)),
+    ]
+
+
 class PlyInfo(C.Structure):
     _fields_ = [
         ("num_splats", C.c_uint32),
@@ -364,6 +386,24 @@ SIGNATURES = {
     "bsx_mean_noise_step": (
         C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_float, C.c_float, C.c_uint64,
                   C.c_uint32]
+    ),
+    "bsx_dropout_fwd": (
+        C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_int32, C.POINTER(DropoutCfg), C.c_void_p,
+                  C.c_void_p]
+    ),
+    "bsx_dropout_bwd": (
+        C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_int32, C.POINTER(DropoutCfg), C.c_void_p, C.c_void_p]
+    ),
+    "bsx_group_norm_workspace": (
+        C.c_int, [C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int32, C.POINTER(C.c_uint64)]
+    ),
+    "bsx_group_norm_fwd": (
+        C.c_int, [C.c_void_p] * 4 + [C.c_uint64, C.c_uint64, C.c_uint32, C.c_int32, C.POINTER(GroupNormCfg)] +
+        [C.c_void_p] * 4 + [C.c_uint64, C.c_void_p]
+    ),
+    "bsx_group_norm_bwd": (
+        C.c_int, [C.c_void_p] * 7 + [C.c_uint64, C.c_uint64, C.c_uint32, C.c_int32, C.POINTER(GroupNormCfg)] +
+        [C.c_void_p] * 4 + [C.c_uint64, C.c_void_p]
     ),
     "bsx_radix_argsort_u32": (
         C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p]

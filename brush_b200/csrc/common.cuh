@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <map>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -158,6 +159,8 @@ struct bsx_ctx {
         // percentile bounds of the means (bounds.cu)
         bounds_tmp;
     bsx_fwd_state fwd;
+    // the feature operators (dropout.cu, group_norm.cu) may be called from several threads at once
+    std::mutex op_mutex;
     // optional per-launch timing (bsx_profile_*)
     int profiling = 0;
     cudaEvent_t prof_start = nullptr;
@@ -183,6 +186,9 @@ void release(bsx_ctx* ctx, DevBuf& b);
 void prof_begin(bsx_ctx* ctx);
 // Checks the launch that was just enqueued and counts it.
 bsx_status post_launch(bsx_ctx* ctx, const char* name);
+// The same two for a launch on a stream other than the context's.
+void prof_begin_on(bsx_ctx* ctx, cudaStream_t stream);
+bsx_status post_launch_on(bsx_ctx* ctx, const char* name, cudaStream_t stream);
 // Reads and clears the device error word (synchronises the stream).
 bsx_status check_device_error(bsx_ctx* ctx);
 

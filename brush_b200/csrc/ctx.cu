@@ -55,17 +55,18 @@ static cudaEvent_t pool_event(bsx_ctx* ctx) {
     return e;
 }
 
-void prof_begin(bsx_ctx* ctx) {
+void prof_begin_on(bsx_ctx* ctx, cudaStream_t stream) {
     if (!ctx->profiling) return;
     ctx->prof_start = pool_event(ctx);
-    cudaEventRecord(ctx->prof_start, ctx->stream);
+    cudaEventRecord(ctx->prof_start, stream);
 }
+void prof_begin(bsx_ctx* ctx) { prof_begin_on(ctx, ctx->stream); }
 
-bsx_status post_launch(bsx_ctx* ctx, const char* name) {
+bsx_status post_launch_on(bsx_ctx* ctx, const char* name, cudaStream_t stream) {
     ctx->launches++;
     if (ctx->profiling && ctx->prof_start) {
         cudaEvent_t end = pool_event(ctx);
-        cudaEventRecord(end, ctx->stream);
+        cudaEventRecord(end, stream);
         ctx->prof_pending.push_back({name, ctx->prof_start, end});
         ctx->prof_start = nullptr;
     }
@@ -73,6 +74,7 @@ bsx_status post_launch(bsx_ctx* ctx, const char* name) {
     if (e != cudaSuccess) return fail(ctx, BSX_ERR_CUDA, std::string("launch of ") + name + ": " + cudaGetErrorString(e));
     return BSX_OK;
 }
+bsx_status post_launch(bsx_ctx* ctx, const char* name) { return post_launch_on(ctx, name, ctx->stream); }
 
 bsx_status check_device_error(bsx_ctx* ctx) {
     cudaError_t e = cudaMemcpyAsync(ctx->h_pinned + 8, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream);
@@ -219,6 +221,7 @@ bsx_status bsx_profile_collect(bsx_ctx* ctx) {
     if (s != BSX_OK) return s;
     for (auto& r : ctx->prof_pending) {
         float ms = 0.0f;
+        cudaEventSynchronize(r.b);  // launches on other streams
         cudaEventElapsedTime(&ms, r.a, r.b);
         size_t i = 0;
         while (i < ctx->prof_names.size() && ctx->prof_names[i] != r.name) ++i;

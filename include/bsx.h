@@ -570,6 +570,80 @@ BSX_API bsx_status bsx_mean_noise_step(bsx_ctx* ctx, float* d_transforms, const 
                                        const float* d_gate, uint32_t num_splats, float scale, float limit,
                                        uint64_t seed, uint32_t step);
 
+/* ---- feature operators: dropout and group norm, channels last ----
+ * No counterpart in the reference. They serve training next to the renderer: splats or
+ * features dropped at random (beside the mean noise above), and learned networks on
+ * channels-last images such as the renders. Unlike the calls above they take their stream
+ * as an argument, keep nothing in the context but its error text, launch count and launch
+ * times, and need no memory beyond what the caller passes: calls on several streams, from
+ * several threads and inside stream capture may overlap. Tensors are contiguous, need no
+ * alignment beyond their element's (16 bytes is faster), and their element type is one
+ * of bsx_dtype; sums, statistics and products are formed in 32 bits and rounded once. */
+typedef enum bsx_dtype { BSX_F32 = 0, BSX_BF16 = 1, BSX_F16 = 2 } bsx_dtype;
+
+/* Dropout with a counter-based mask that is never stored. Element i uses draw m = i / share
+ * (share = 1: a draw for each element; share = the row length: rows dropped as a whole).
+ * Draws come from Philox-4x32 with 7 rounds, key = (seed low, seed high), counter =
+ * (q low, q high, step, half) with q = m / 8: halfword m % 8 of the block (low half of
+ * word 0, high half of word 0, low half of word 1, ...) with half = 0 gives the high 16
+ * bits of a 32-bit draw, with half = 1 the low 16 bits. Element i is kept when its draw is
+ * >= rint(p 2^32) (ties to even), and then scaled by 1 / (1 - p); a dropped element is 0
+ * whatever it held. p = 0 keeps and p = 1 drops everything. With d_step the step is read
+ * on the device when the kernel runs, so that a captured graph can draw a new mask at each
+ * replay. */
+typedef struct bsx_dropout_cfg {
+    double p;                /* in [0, 1] */
+    uint64_t seed;
+    uint64_t share;          /* consecutive elements that share a draw, >= 1 */
+    const uint32_t* d_step;  /* device; null: step */
+    uint32_t step;
+} bsx_dropout_cfg;
+/* out = residual + dropout(x); d_residual may be null. d_out may be d_x or d_residual
+ * (other overlaps are undefined). */
+BSX_API bsx_status bsx_dropout_fwd(bsx_ctx* ctx, const void* d_x, const void* d_residual, uint64_t count,
+                                   int32_t dtype, const bsx_dropout_cfg* cfg, void* d_out, void* cuda_stream);
+/* v_x from v_out, with the mask drawn again; the residual's gradient is v_out itself.
+ * d_v_x may be d_v_out. */
+BSX_API bsx_status bsx_dropout_bwd(bsx_ctx* ctx, const void* d_v_out, uint64_t count, int32_t dtype,
+                                   const bsx_dropout_cfg* cfg, void* d_v_x, void* cuda_stream);
+
+typedef enum bsx_activation {
+    BSX_ACT_NONE = 0,
+    BSX_ACT_SILU = 1,     /* z sigmoid(z) */
+    BSX_ACT_GELU_TANH = 2 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+} bsx_activation;
+
+/* Group norm of x [N, pixels, C], channels last: for sample n and group g of C / groups
+ * channels, mean and biased variance over the group's pixels and channels, rstd =
+ * 1 / sqrt(var + eps), z = weight[c] (x - mean) rstd + bias[c], out = dropout(act(z)).
+ * weight and bias may be null (1 and 0) and have type param_dtype (x's type or BSX_F32);
+ * dropout may be null, its share must be 1, and it draws the mask that bsx_dropout_fwd
+ * draws for the same output tensor. mean and rstd [N, groups] are float. */
+typedef struct bsx_group_norm_cfg {
+    uint32_t groups;
+    float eps;
+    int32_t activation;   /* bsx_activation */
+    int32_t param_dtype;  /* bsx_dtype */
+    const bsx_dropout_cfg* dropout;
+} bsx_group_norm_cfg;
+/* Bytes of workspace that a forward (backward = 0) or backward call with these sizes needs. */
+BSX_API bsx_status bsx_group_norm_workspace(uint64_t n, uint64_t pixels, uint32_t channels, uint32_t groups,
+                                            int32_t backward, uint64_t* bytes);
+/* d_workspace: 16-byte aligned, its contents do not matter and nothing is kept in it; calls
+ * that may overlap need one each. No output may overlap an input. */
+BSX_API bsx_status bsx_group_norm_fwd(bsx_ctx* ctx, const void* d_x, const void* d_weight, const void* d_bias,
+                                      uint64_t n, uint64_t pixels, uint32_t channels, int32_t dtype,
+                                      const bsx_group_norm_cfg* cfg, void* d_out, float* d_mean, float* d_rstd,
+                                      void* d_workspace, uint64_t workspace_bytes, void* cuda_stream);
+/* Gradients of bsx_group_norm_fwd for v_out, with the forward's inputs and its mean and
+ * rstd: v_x [N, pixels, C], v_weight and v_bias [C] (param_dtype; each may be null). z, the
+ * activation and the mask are formed again. Results do not depend on scheduling. */
+BSX_API bsx_status bsx_group_norm_bwd(bsx_ctx* ctx, const void* d_v_out, const void* d_x, const void* d_weight,
+                                      const void* d_bias, const float* d_mean, const float* d_rstd, uint64_t n,
+                                      uint64_t pixels, uint32_t channels, int32_t dtype,
+                                      const bsx_group_norm_cfg* cfg, void* d_v_x, void* d_v_weight, void* d_v_bias,
+                                      void* d_workspace, uint64_t workspace_bytes, void* cuda_stream);
+
 /* ---- primitives: brush-sort / brush-prefix-sum / get_tile_offsets ---- */
 /* Stable argsort by key & mask(bits rounded up to a multiple of 4), as
  * crates/brush-sort/src/lib.rs:16-129. Inputs are left untouched. */
