@@ -4,8 +4,8 @@ Each translation unit is compiled by nvcc in parallel and linked in-tree so the
 library travels with the source tree. Floating-point contraction is disabled
 (``-fmad=false``, ``-ffp-contract=off``): the pipeline's discrete decisions
 (culling, tile counts, alpha cutoffs) must be reproducible bit-for-bit by a
-host restatement compiled the same way. The image loss, checked by tolerance
-and free of such decisions, is compiled with contraction (``CONTRACTED``).
+host restatement compiled the same way. The image loss and group norm, checked by
+tolerance and free of such decisions, are compiled with contraction (``CONTRACTED``).
 """
 from __future__ import annotations
 
@@ -51,7 +51,7 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 # unit keeps exact IEEE operations, because the CPU oracle (g++ -ffp-contract=off)
 # restates its decisions (culling, tile counts, alpha and early-out tests, the
 # raster backward's replay of the forward) or its results bit for bit.
-CONTRACTED = {"loss.cu"}
+CONTRACTED = {"loss.cu", "group_norm_f32.cu", "group_norm_bf16.cu", "group_norm_f16.cu"}
 
 
 def _compile(src: Path, verbose: bool) -> Path:

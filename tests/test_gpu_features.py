@@ -383,6 +383,13 @@ def test_group_norm_far_elements(cuda):
     """Offsets beyond 2^31 elements: the last sample equals the same sample alone."""
     import brush_b200 as bsx
 
+    def step_apart(a, b):
+        # the two split their sums differently, so their 32-bit values differ by far less than a bf16 step (2^-7 of
+        # the value at most) and round to the same number or to neighbours
+        a, b = a.float(), b.float()
+        return bool(((a - b).abs() <= 2.0**-7 * torch.maximum(a.abs(), b.abs()) + 1e-4).all())
+
+    torch.manual_seed(0)
     n, px, c = 33, 1 << 20, 64  # 2.2e9 elements
     one = torch.randn(1, px, c, device="cuda").bfloat16()
     x = one.expand(n, px, c).contiguous()
@@ -395,11 +402,11 @@ def test_group_norm_far_elements(cuda):
     m64 = x64.mean((0, 2))
     assert (mean.double() - m64).abs().max() <= 1e-5 and (mean[-1] - want[1][0]).abs().max() <= 1e-6
     assert (rstd[-1] / want[2][0] - 1).abs().max() <= 1e-5
-    assert (out[-1].float() - want[0][0].float()).abs().max() <= 0.05 and torch.equal(out[-1, -1].isnan(), out[0, 0].isnan())
+    assert step_apart(out[-1], want[0][0])
     del out
     v_x, v_w, v_b = bsx.group_norm_backward(v, x, w, b, mean, rstd, cfg)
     g = bsx.group_norm_backward(v[:1], one, w, b, mean[:1].contiguous(), rstd[:1].contiguous(), cfg)
-    assert (v_x[-1].float() - g[0][0].float()).abs().max() <= 0.05
+    assert step_apart(v_x[-1], g[0][0])
     assert (v_w / n - g[1]).abs().max() <= 1e-3 * g[1].abs().max()
     del x, v, v_x
     torch.cuda.empty_cache()
@@ -427,7 +434,7 @@ def test_group_norm_entry_point_errors(cuda, bsx_lib):
     from brush_b200._context import context
 
     ctx, L = context(0), bsx_lib.lib()
-    x = torch.zeros(2 * 16 * 8, device="cuda")
+    x = torch.zeros(2 * 9000 * 8, device="cuda")
     ws = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
     st = torch.zeros(64, device="cuda")
     s = torch.cuda.current_stream().cuda_stream
@@ -444,7 +451,9 @@ def test_group_norm_entry_point_errors(cuda, bsx_lib):
     for kw, want in [(dict(g=3), 2), (dict(g=0), 2), (dict(c=0), 2), (dict(px=0), 2), (dict(n=1 << 31), 2),
                      (dict(px=1 << 62), 2), (dict(eps=-1.0), 1), (dict(act=3), 1), (dict(pt=1), 1), (dict(t=3), 1),
                      (dict(t=-1), 1), (dict(xp=None), 1), (dict(xp=x.data_ptr() + 2), 1),
-                     (dict(wsp=ws.data_ptr() + 4), 1), (dict(wsn=0), 3), (dict(wsp=None), 3)]:
+                     (dict(wsp=ws.data_ptr() + 4), 1),
+                     # samples that a block holds need no workspace in the forward; these do
+                     (dict(wsn=0, px=9000), 3), (dict(wsp=None, px=9000), 3)]:
         assert call(**kw) == want, kw
         assert L.bsx_last_error(ctx.handle)
     ctx.sync()
