@@ -41,38 +41,48 @@ uint32_t groups_of_tile(uint32_t c, uint32_t per, uint32_t channels, uint32_t ti
     return (channels - 1) / per + 2;  // cut groups at both ends
 }
 
-// The cut for vectors of v elements; v divides a sample.
-Plan plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t v, bool bwd) {
+// The cut for vectors of v elements; v divides a sample. False: more rows than the kernels count.
+bool plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t v, bool bwd, Plan& p) {
     const uint32_t per = c / groups, batch = bwd ? kBatchBwd : kBatch;
-    Plan p{};
+    p = Plan{};
     p.v = v;
-    p.rv = c / std::gcd(c, v);
     p.vecs = pixels * c / v;
-    p.rows = (p.vecs + p.rv - 1) / p.rv;
-    p.cols = p.rv < (uint32_t)kThreads ? p.rv : kThreads;
-    p.tiles = (p.rv + p.cols - 1) / p.cols;
-    p.k = kThreads / p.cols;
-    // Small: a block holds a (sample, tile) in registers. Tiles of whole groups, half a sector of a row at least.
-    const auto fits = [&](uint32_t cols) { return cols <= (uint32_t)kThreads && p.rows <= (uint64_t)(kThreads / cols) * batch; };
-    if (fits(p.rv)) {
-        p.small = 1;
+    p.by_per = Div32::of(per, c);
+    p.by_c = Div32::of(c, (uint64_t)kThreads * 8);
+    const uint32_t run = c / std::gcd(c, v);  // the shortest row
+    const uint64_t rows = (p.vecs + run - 1) / run;
+    // Small: a block holds a (sample, tile) in registers. Tiles are whole groups and at least half a sector wide.
+    const auto fits = [&](uint64_t cols) { return cols <= (uint64_t)kThreads && rows <= (kThreads / cols) * batch; };
+    uint64_t cols = 0;
+    if (fits(run)) {
+        cols = run;
     } else if (c % v == 0) {
-        const uint64_t unit = std::lcm((uint64_t)per, (uint64_t)v) / v;  // vectors
-        uint64_t cols = 0;
-        if (unit <= (uint64_t)kThreads && fits((uint32_t)unit)) cols = unit;
-        while (cols && cols + unit <= (uint64_t)kThreads && cols + unit < p.rv && fits((uint32_t)(cols + unit))) cols += unit;
-        if (cols * v >= 16 && (p.rv + cols - 1) / cols <= 64) {
-            p.small = 1;
-            p.cols = (uint32_t)cols;
-            p.tiles = (uint32_t)((p.rv + cols - 1) / cols);
-            p.k = kThreads / p.cols;
-        }
+        const uint64_t unit = std::lcm((uint64_t)per, (uint64_t)v) / v;
+        if (fits(unit)) cols = unit;
+        while (cols && cols + unit < run && fits(cols + unit)) cols += unit;
+        if (cols * v < 16 || (run + cols - 1) / (cols ? cols : 1) > 64) cols = 0;
     }
-    if (p.small && p.k > p.rows) p.k = (uint32_t)p.rows;
+    if (cols) {
+        p.small = 1;
+        p.rv = run;
+        p.rows = (uint32_t)rows;
+        p.cols = (uint32_t)cols;
+        p.k = kThreads / p.cols < p.rows ? kThreads / p.cols : p.rows;
+    } else {
+        p.rv = run < (uint32_t)kThreads ? kThreads / run * run : run;
+        const uint64_t wide = (p.vecs + p.rv - 1) / p.rv;
+        if (wide >= 1ull << 31) return false;
+        p.rows = (uint32_t)wide;
+        p.cols = p.rv < (uint32_t)kThreads ? p.rv : kThreads;
+        p.k = 1;
+    }
+    p.last = (uint32_t)(p.vecs - (uint64_t)(p.rows - 1) * p.rv);
+    p.tiles = (p.rv + p.cols - 1) / p.cols;
     p.threads = (p.k * p.cols + 31) / 32 * 32;
     p.blocks = p.small ? (uint32_t)(n * p.tiles) : 0;
     p.gl = groups_of_tile(c, per, p.cols * v, p.tiles);
-    return p;
+    p.by_cols = Div32::of(p.cols, kThreads);
+    return p.small || (uint64_t)p.rows * n * p.tiles < 1ull << 31;
 }
 
 // Floats of workspace: the partial sums that plan_for's kernels leave (group_norm_fwd.cuh, group_norm_bwd.cuh).
@@ -90,9 +100,10 @@ bool usable(uint64_t pixels, uint32_t c, uint32_t v) {
 
 uint64_t workspace_floats(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, bool bwd) {
     uint64_t most = 0;  // of the cuts that type and alignment may choose
+    Plan p;
     for (uint32_t v : {8u, 4u, 2u, 1u})
-        if (usable(pixels, c, v)) {
-            const uint64_t w = workspace_of(plan_for(n, pixels, c, groups, v, bwd), n, c, bwd);
+        if (usable(pixels, c, v) && plan_for(n, pixels, c, groups, v, bwd, p)) {
+            const uint64_t w = workspace_of(p, n, c, bwd);
             if (w > most) most = w;
         }
     return most;
@@ -143,7 +154,8 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
         const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.v | (uintptr_t)a.out;
         uint32_t v = 16 / (uint32_t)size;
         if (all % 16 || !usable(a.pixels, a.c, v)) v = size == 2 && all % 4 == 0 && usable(a.pixels, a.c, 2) ? 2 : 1;
-        Plan p = plan_for(a.n, a.pixels, a.c, a.groups, v, bwd);
+        Plan p;
+        if (!plan_for(a.n, a.pixels, a.c, a.groups, v, bwd, p)) return fail(ctx, BSX_ERR_CAPACITY, "too many rows");
         const Call call{&a, &p, cfg->activation, drop, a.per % v == 0, bwd, ctx->device, st};
         prof_begin_on(ctx, st);
         const cudaError_t e = dtype == BSX_F32 ? launch<float>(call) : dtype == BSX_BF16 ? launch<__nv_bfloat16>(call) : launch<__half>(call);

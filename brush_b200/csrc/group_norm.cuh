@@ -1,11 +1,12 @@
 // group_norm.cuh - what the group-norm kernels share: arguments, the cut of a tensor into
-// blocks, per-thread statistics, sums over groups inside a block, and the activation.
+// blocks, sums over groups inside a block, and the activation.
 //
-// Layout. A sample is a run of pixels C elements long. Threads read vectors of V elements; a
-// "row" is the shortest run that starts and ends on a pixel and on a vector: C / gcd(C, V)
-// vectors, lcm(C, V) elements. A block takes k rows at a time with one vector a thread, so a
-// thread meets the same V channels in every row: their weights, biases and statistics stay in
-// its registers, odd channel counts included. Wide rows are cut into tiles of columns.
+// Layout. A sample is a run of pixels C elements long, read in vectors of V elements. The
+// shortest run that starts and ends on a pixel and on a vector has C / gcd(C, V) vectors. A
+// "row" is such a run, or for large samples as many of them as a block takes at once, one
+// vector a thread: a thread meets the same V channels in every row, so that their weights,
+// biases and statistics stay in its registers, odd channel counts included. Rows wider than a
+// block, and rows of many channels in small samples, are cut into tiles of columns.
 #pragma once
 
 #include "dropout.cuh"
@@ -14,12 +15,22 @@
 namespace bsx {
 namespace norm {
 
-constexpr int kThreads = 512;     // most threads of a block
-constexpr int kBatch = 8;         // vectors of a thread in the kernels for small samples
-constexpr int kFlight = 4;        // vectors of a thread in flight in the kernels for large samples
-constexpr int kBatchBwd = 4;      // the same two for the backward, of x and of v each
-constexpr int kFlightBwd = 2;
-constexpr uint32_t kMaxBlocks = 512;  // most blocks of a kernel for large samples
+constexpr int kThreads = 512;         // most threads of a block
+constexpr int kBatch = 8;             // vectors a thread holds, small samples
+constexpr int kFlight = 8;            // rows in flight ahead of the one at work, large samples
+constexpr int kBatchBwd = 4;          // the same two for the backward, of x and of v each
+constexpr int kFlightBwd = 5;
+constexpr uint32_t kMaxBlocks = 512;  // most blocks of a kernel that leaves partial sums
+
+// Division of x by d for x d < 2^32: with f = (2^32 + e) / d, 0 < e <= d, the product's high word is
+// floor(x / d + x e / (d 2^32)), and the second term stays below 1 / d. Beyond, a plain division.
+struct Div32 {
+    uint32_t d, f;
+    static Div32 of(uint32_t d, uint64_t most) { return {d, d > 1 && most * d < (1ull << 32) ? (uint32_t)((1ull << 32) / d + 1) : 0}; }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+        return f ? __umulhi(x, f) : d == 1 ? x : x / d;
+    }
+};
 
 struct Args {
     const void* x;
@@ -42,17 +53,20 @@ struct Args {
 // How the tensor is cut (plan_for in group_norm.cu).
 struct Plan {
     uint64_t vecs;       // vectors of a sample
-    uint64_t rows;       // rows of a sample; the last may be cut short
-    uint64_t per_block;  // large samples: rows of a block, over tiles and samples in order
+    uint32_t rows;       // rows of a sample
+    uint32_t last;       // vectors of its last row
     uint32_t rv;         // vectors of a row
     uint32_t cols;       // vectors of a tile's row; the last tile may have fewer
     uint32_t tiles;
-    uint32_t k;          // rows a block takes at a time
+    uint32_t k;          // small samples: rows a block takes at a time
     uint32_t gl;         // most groups of a tile
-    uint32_t keep;       // large samples: iterations whose vectors stay in shared memory
+    uint32_t per_block;  // large samples: rows of a block
+    uint32_t per_unit;   // blocks of a (tile, sample); 0: the rows of all of them are dealt to the blocks in order
+    uint32_t ring;       // rows in shared memory
     uint32_t threads, blocks;
     uint32_t v;          // elements of a vector
     int small;           // one block per (sample, tile), everything in registers
+    Div32 by_cols, by_per, by_c;
 };
 
 template <class T>
@@ -60,145 +74,165 @@ __device__ __forceinline__ float param(const void* p, int f32, uint32_t c, float
     if (!p) return without;
     return f32 ? __ldg((const float*)p + c) : to_f(((const T*)p)[c]);
 }
+// Of V channels from c on; wrap: they may run past the last channel (rows of several pixels).
+template <class T, int V>
+__device__ __forceinline__ void params(const Args& a, const void* p, uint32_t c, bool wrap, float without, float (&to)[V]) {
+    if (V > 1 && !wrap && p && (uintptr_t)p % 16 == 0) {
+        if (a.param_f32) {
+            Pack<float, V> raw;
+            raw.load((const float*)p + c);
+            raw.get(to);
+        } else {
+            Pack<T, V> raw;
+            raw.load((const T*)p + c);
+            raw.get(to);
+        }
+        return;
+    }
+    uint32_t ch = c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        to[j] = param<T>(p, a.param_f32, ch, without);
+        if (++ch == a.c) ch = 0;
+    }
+}
 
+// Two 32-bit lanes in one instruction, each rounded as the scalar one.
+__device__ __forceinline__ void fma2(float& r0, float& r1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;}"
+        : "=f"(r0), "=f"(r1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float& r0, float& r1, float a0, float a1, float b0, float b1) {
+    asm("{.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;}"
+        : "=f"(r0), "=f"(r1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float& r0, float& r1, float a0, float a1, float b0, float b1) {
+    asm("{.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;}"
+        : "=f"(r0), "=f"(r1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+// r = a b + c, a b, a + b over V lanes; the operands of fewer lanes repeat.
+template <int V, int A, int B, int C>
+__device__ __forceinline__ void fma_v(float (&r)[V], const float (&a)[A], const float (&b)[B], const float (&c)[C]) {
+    if constexpr (V == 1) r[0] = __fmaf_rn(a[0], b[0], c[0]);
+    else
+#pragma unroll
+        for (int j = 0; j < V; j += 2)
+            fma2(r[j], r[j + 1], a[j % A], a[(j + 1) % A], b[j % B], b[(j + 1) % B], c[j % C], c[(j + 1) % C]);
+}
+template <int V, int A, int B>
+__device__ __forceinline__ void mul_v(float (&r)[V], const float (&a)[A], const float (&b)[B]) {
+    if constexpr (V == 1) r[0] = __fmul_rn(a[0], b[0]);
+    else
+#pragma unroll
+        for (int j = 0; j < V; j += 2) mul2(r[j], r[j + 1], a[j % A], a[(j + 1) % A], b[j % B], b[(j + 1) % B]);
+}
+template <int V, int A, int B>
+__device__ __forceinline__ void add_v(float (&r)[V], const float (&a)[A], const float (&b)[B]) {
+    if constexpr (V == 1) r[0] = __fadd_rn(a[0], b[0]);
+    else
+#pragma unroll
+        for (int j = 0; j < V; j += 2) add2(r[j], r[j + 1], a[j % A], a[(j + 1) % A], b[j % B], b[(j + 1) % B]);
+}
+// sum[j % A] += v[j] and sum[j % A] += a[j] b[j]: A partial sums.
+template <int V, int A>
+__device__ __forceinline__ void accumulate(float (&sum)[A], const float (&v)[V]) {
+    if constexpr (A == 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[0] += v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 2)
+            add2(sum[j % A], sum[(j + 1) % A], sum[j % A], sum[(j + 1) % A], v[j], v[j + 1]);
+    }
+}
+template <int V, int A>
+__device__ __forceinline__ void accumulate(float (&sum)[A], const float (&a)[V], const float (&b)[V]) {
+    if constexpr (A == 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[0] = __fmaf_rn(a[j], b[j], sum[0]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 2)
+            fma2(sum[j % A], sum[(j + 1) % A], a[j], a[j + 1], b[j], b[j + 1], sum[j % A], sum[(j + 1) % A]);
+    }
+}
+// Partial sums that keep the lanes of a pair apart.
+template <int V, int L>
+constexpr int kParts = L > 1 ? V : V > 1 ? 2 : 1;
+// One sum per item from them.
+template <int V, int L>
+__device__ __forceinline__ void per_item(const float (&part)[kParts<V, L>], float (&item)[L]) {
+    if constexpr (L > 1 || V == 1) {
+#pragma unroll
+        for (int j = 0; j < L; ++j) item[j] = part[j];
+    } else {
+        item[0] = part[0] + part[1];
+    }
+}
+
+// The approximate exponential and reciprocal (2 and 1 ulp); results below 2^-126 become 0.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float rcp_fast(float x) {
     float y;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
 // act(z) = z s(w(z)), s the logistic function: w = z (silu), or 2 sqrt(2/pi) (z + 0.044715 z^3)
-// (gelu in its tanh form, because (1 + tanh(t)) / 2 = s(2 t)). s = 1 / (1 + 2^(-w log2 e)), with
-// the approximate exponential and reciprocal (2 and 1 ulp); both ends are right: the exponential
-// overflows to infinity and s to 0, or vanishes and s is 1.
+// (gelu in its tanh form, because (1 + tanh(t)) / 2 = s(2 t)). s = 1 / (1 + 2^(-w log2 e)); both
+// ends are right: the exponential overflows to infinity and s is 0, or it vanishes and s is 1.
 constexpr float kLog2e = 1.4426950408889634f, kGelu1 = 1.5957691216057308f, kGelu3 = 0.044715f;
-template <int ACT>
-__device__ __forceinline__ float gate(float z) {
-    if (ACT == BSX_ACT_NONE) return 1.0f;
-    float e;
-    if (ACT == BSX_ACT_SILU) e = z * -kLog2e;
-    else e = z * __fmaf_rn(z * z, -kLog2e * kGelu1 * kGelu3, -kLog2e * kGelu1);
-    return rcp_fast(1.0f + exp2_fast(e));
-}
-template <int ACT>
-__device__ __forceinline__ float act(float z) {
-    return ACT == BSX_ACT_NONE ? z : z * gate<ACT>(z);
-}
-// act'(z) = s + z s (1 - s) w'(z)
-template <int ACT>
-__device__ __forceinline__ float act_grad(float z) {
-    if (ACT == BSX_ACT_NONE) return 1.0f;
-    const float s = gate<ACT>(z);
-    float dw = z;
-    if (ACT == BSX_ACT_GELU_TANH) dw = z * __fmaf_rn(z * z, 3.0f * kGelu1 * kGelu3, kGelu1);
-    return __fmaf_rn(__fmaf_rn(-s, s, s), dw, s);
-}
-
-// The columns and groups of a tile. Items are vectors where a vector lies in one group (L = 1), else elements.
-struct Tile {
-    uint32_t cols;         // vectors in the tile's row
-    uint32_t c0, c1;       // channels
-    uint32_t g0, groups;   // groups that have channels here
-    uint32_t stride;       // items from a channel to its next copy in the block
-    uint32_t copies;       // copies of the channels in the block's k rows
-};
-template <int V, int L>
-__device__ __forceinline__ Tile tile_of(const Args& a, const Plan& p, uint32_t t) {
-    Tile r;
-    r.cols = min(p.cols, p.rv - t * p.cols);
-    if (p.tiles == 1) r.c0 = 0, r.c1 = a.c;
-    else r.c0 = t * p.cols * V, r.c1 = r.c0 + r.cols * V;
-    r.g0 = r.c0 / a.per;
-    r.groups = (r.c1 - 1) / a.per - r.g0 + 1;
-    r.stride = (r.c1 - r.c0) / (V / L);
-    r.copies = p.k * r.cols * L / r.stride;
-    return r;
-}
-
-// Sums over the tile's groups of one value per item (thread t holds items t L ... t L + L - 1 of the block's
-// k rows), in a fixed order: a warp, or several where groups are few, walks each group's items. After the
-// call sum[g] holds group g0 + g for all threads. Starts and ends with a barrier.
-template <int V, int L, bool PAIR>
-__device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const float (&x)[L], const float (&y)[L],
-                                           bool active, float* part, float* warp_sum, float2* sum) {
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    const uint32_t half = blockDim.x * L;  // the pair's second values
-    __syncthreads();
+template <int ACT, int V>
+__device__ __forceinline__ void gates(const float (&z)[V], float (&s)[V]) {
+    constexpr float one[1] = {1.0f};
+    if (ACT == BSX_ACT_SILU) {
+        constexpr float k[1] = {-kLog2e};
+        mul_v<V>(s, z, k);
+    } else {
+        constexpr float k1[1] = {-kLog2e * kGelu1}, k3[1] = {-kLog2e * kGelu1 * kGelu3};
+        mul_v<V>(s, z, z);
+        fma_v<V>(s, s, k3, k1);
+        mul_v<V>(s, s, z);
+    }
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-        part[tid * L + j] = active ? x[j] : 0.0f;
-        if (PAIR) part[half + tid * L + j] = active ? y[j] : 0.0f;
-    }
-    __syncthreads();
-    const uint32_t share = max(1u, warps / t.groups);  // warps of a group
-    for (uint32_t u = warp; u < t.groups * share; u += warps) {
-        const uint32_t g = u / share, q = u - g * share;
-        const uint32_t lo = (max((t.g0 + g) * a.per, t.c0) - t.c0) / (V / L);
-        const uint32_t hi = (min((t.g0 + g + 1) * a.per, t.c1) - t.c0) / (V / L);
-        const uint32_t width = hi - lo, count = t.copies * width;
-        const float inv = 1.0f / (float)width;
-        float s = 0.0f, s2 = 0.0f;
-        for (uint32_t i = q * 32 + lane; i < count; i += 32 * share) {
-            const uint32_t m = (uint32_t)(((float)i + 0.5f) * inv);  // i / width: i < 2^13, far from a whole number
-            const uint32_t at = m * t.stride + lo + (i - m * width);
-            s += part[at];
-            if (PAIR) s2 += part[half + at];
-        }
+    for (int j = 0; j < V; ++j) s[j] = exp2_fast(s[j]);
+    add_v<V>(s, s, one);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            s += __shfl_xor_sync(~0u, s, o);
-            if (PAIR) s2 += __shfl_xor_sync(~0u, s2, o);
-        }
-        if (lane == 0) {
-            warp_sum[u * 2] = s;
-            warp_sum[u * 2 + 1] = s2;
-        }
-    }
-    __syncthreads();
-    for (uint32_t g = tid; g < t.groups; g += blockDim.x) {
-        float s = 0.0f, s2 = 0.0f;
-        for (uint32_t q = 0; q < share; ++q) {
-            s += warp_sum[(g * share + q) * 2];
-            s2 += warp_sum[(g * share + q) * 2 + 1];
-        }
-        sum[g] = make_float2(s, s2);
-    }
-    __syncthreads();
+    for (int j = 0; j < V; ++j) s[j] = rcp_fast(s[j]);
 }
-
-// Floats of shared memory that group_sums takes: part, warp_sum, sum.
-inline uint32_t sums_floats(uint32_t threads, uint32_t lanes, uint32_t gl, bool pair) {
-    return threads * lanes * (pair ? 2 : 1) + 2 * (gl > kThreads / 32 ? gl : kThreads / 32) + 2 * gl;
-}
-template <int L, bool PAIR>
-struct Scratch {
-    float *part, *warp_sum;
-    float2* sum;
-    float* end;
-    __device__ __forceinline__ Scratch(float* smem, uint32_t gl) {
-        part = smem;
-        warp_sum = part + blockDim.x * L * (PAIR ? 2 : 1);
-        sum = (float2*)(warp_sum + 2 * max(gl, (uint32_t)kThreads / 32));
-        end = (float*)(sum + gl);
+template <int ACT, int V>
+__device__ __forceinline__ void activate(float (&z)[V]) {
+    if constexpr (ACT != BSX_ACT_NONE) {
+        float s[V];
+        gates<ACT>(z, s);
+        mul_v<V>(z, z, s);
     }
-};
-
-// Group of lane j of a vector that starts at channel c, relative to the tile's first.
-template <int V, int L>
-__device__ __forceinline__ uint32_t group_at(const Args& a, const Tile& t, uint32_t c, int j) {
-    uint32_t ch = c + j;
-    if (L > 1) while (ch >= a.c) ch -= a.c;  // rows of several pixels
-    return ch / a.per - t.g0;
 }
-__device__ __forceinline__ uint32_t channel_at(const Args& a, uint32_t c, int j) {
-    uint32_t ch = c + j;
-    while (ch >= a.c) ch -= a.c;
-    return ch;
+// act'(z) = s + (s - s^2) z w'(z)
+template <int ACT, int V>
+__device__ __forceinline__ void slopes(float (&z)[V]) {
+    float s[V], t[V], neg[V];
+    gates<ACT>(z, s);
+    if (ACT == BSX_ACT_GELU_TANH) {
+        constexpr float k1[1] = {kGelu1}, k3[1] = {3.0f * kGelu1 * kGelu3};
+        mul_v<V>(t, z, z);
+        fma_v<V>(t, t, k3, k1);
+        mul_v<V>(z, z, t);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) neg[j] = -s[j];
+    fma_v<V>(t, neg, s, s);
+    fma_v<V>(z, t, z, s);
 }
 
 // drop for V elements from flat element `at` (V divides it, and 8).
@@ -213,44 +247,255 @@ __device__ __forceinline__ void drop_vector(const DropArgs& d, uint32_t step, ui
     }
 }
 
-// A block's share of one (tile, sample) of a large tensor.
-struct Segment {
-    uint64_t n, r0, at;   // sample, first row, first element of the thread's first vector
-    uint32_t tile, c;     // tile, channel of the thread's first element
-    uint32_t iters, cnt;  // iterations of the block, of this thread
-    uint32_t pixels;      // float-exact below 2^24; counts enter as float
+// The columns and groups of a tile. Items are vectors where a vector lies in one group (L = 1), else elements.
+struct Tile {
+    uint32_t cols;         // vectors in the tile's row
+    uint32_t c0, c1;       // channels
+    uint32_t g0, groups;   // groups that have channels here
+    uint32_t stride;       // items from a channel to its next copy in the block
+    uint32_t copies;       // copies of the channels in the block's k rows
+    uint32_t lanes, log;   // threads that add up a group: 2^log
 };
-__device__ __forceinline__ uint32_t segment_iters(const Plan& p, uint64_t len) { return (uint32_t)((len + p.k - 1) / p.k); }
-
 template <int V, int L>
-__device__ __forceinline__ Segment segment_of(const Args& a, const Plan& p, uint64_t u, uint64_t from, uint64_t to,
-                                              Tile& t) {
-    Segment s;
-    s.tile = (uint32_t)(u / a.n);
-    s.n = u - s.tile * a.n;
-    s.r0 = from - u * p.rows;
-    t = tile_of<V, L>(a, p, s.tile);
-    const uint64_t r1 = to - u * p.rows;
-    const uint32_t tid = threadIdx.x, row = tid / t.cols, col = s.tile * p.cols + tid - row * t.cols;
-    const uint64_t lim = r1 - (r1 == p.rows && (p.rows - 1) * p.rv + col >= p.vecs);  // rows of this column
-    s.iters = segment_iters(p, r1 - s.r0);
-    s.cnt = row < p.k && s.r0 + row < lim ? (uint32_t)((lim - s.r0 - row + p.k - 1) / p.k) : 0;
-    s.at = (s.n * p.vecs + (s.r0 + row) * p.rv + col) * V;
-    s.c = col * V % a.c;
-    const uint64_t e1 = r1 * p.rv * V;
-    s.pixels = (uint32_t)(((e1 < p.vecs * V ? e1 : p.vecs * V) - s.r0 * p.rv * V) / a.c);
-    return s;
+__device__ __forceinline__ Tile tile_of(const Args& a, const Plan& p, uint32_t t) {
+    Tile r;
+    if (p.tiles == 1) {
+        r.cols = p.cols;
+        r.c0 = 0, r.c1 = a.c;
+        r.g0 = 0, r.groups = a.groups;
+        r.stride = a.c / (V / L);
+        r.copies = p.by_c(p.k * p.cols * V);
+    } else {
+        r.cols = min(p.cols, p.rv - t * p.cols);
+        r.c0 = t * p.cols * V, r.c1 = r.c0 + r.cols * V;
+        r.g0 = p.by_per(r.c0);
+        r.groups = p.by_per(r.c1 - 1) - r.g0 + 1;
+        r.stride = r.cols * L;
+        r.copies = p.k;
+    }
+    const uint32_t each = blockDim.x / r.groups;
+    r.log = each ? 31 - __clz(each) : 0;
+    r.lanes = 1u << r.log;
+    return r;
+}
+// Channels of group g0 + q in the tile, in items from c0: [lo, hi).
+template <int V, int L>
+__device__ __forceinline__ void group_span(const Args& a, const Tile& t, uint32_t q, uint32_t& lo, uint32_t& hi) {
+    const uint32_t first = (t.g0 + q) * a.per;
+    lo = (max(first, t.c0) - t.c0) / (V / L);
+    hi = (min(first + a.per, t.c1) - t.c0) / (V / L);
 }
 
-// Iterations of block b's run, over its segments.
-__device__ __forceinline__ uint32_t run_iters(const Plan& p, uint64_t w0, uint64_t w1) {
-    uint32_t all = 0;
-    for (uint64_t w = w0; w < w1;) {
-        const uint64_t next = (w / p.rows + 1) * p.rows, to = next < w1 ? next : w1;
-        all += segment_iters(p, to - w);
-        w = to;
+// Sums over the tile's groups of one value per item (thread t holds items t L ... t L + L - 1 of the block's
+// rows), in a fixed order: t.lanes threads walk each group's items. Afterwards sum[q] holds group g0 + q for all
+// threads. Starts without a barrier (whoever read part or sum last has passed one since, or passes the first one
+// here before they are written); ends with one.
+template <int V, int L, bool PAIR>
+__device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const float (&x)[L], const float (&y)[L],
+                                           bool active, float* part, float2* warp_sum, float2* sum) {
+    const uint32_t tid = threadIdx.x, half = blockDim.x * L;  // half: the pair's second values
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        part[tid * L + j] = active ? x[j] : 0.0f;
+        if (PAIR) part[half + tid * L + j] = active ? y[j] : 0.0f;
     }
-    return all;
+    __syncthreads();
+    const uint32_t in = min(t.lanes, 32u);
+    for (uint32_t base = 0; base < t.groups * t.lanes; base += blockDim.x) {
+        const uint32_t u = base + tid, q = u >> t.log, l = u & (t.lanes - 1);
+        float s = 0.0f, s2 = 0.0f;
+        if (q < t.groups) {
+            uint32_t lo, hi;
+            group_span<V, L>(a, t, q, lo, hi);
+            const uint32_t width = hi - lo;
+            uint32_t m = (uint32_t)(((float)l + 0.5f) / (float)width), i = l - m * width;  // l < 2^9, exact
+            const uint32_t dm = (uint32_t)(((float)t.lanes + 0.5f) / (float)width), di = t.lanes - dm * width;
+            while (m < t.copies) {
+                const uint32_t at = m * t.stride + lo + i;
+                s += part[at];
+                if (PAIR) s2 += part[half + at];
+                m += dm, i += di;
+                if (i >= width) i -= width, ++m;
+            }
+        }
+        for (uint32_t o = in / 2; o; o /= 2) {
+            s += __shfl_xor_sync(~0u, s, o);
+            if (PAIR) s2 += __shfl_xor_sync(~0u, s2, o);
+        }
+        if (t.lanes <= 32) {
+            if (l == 0 && q < t.groups) sum[q] = make_float2(s, s2);
+        } else if ((tid & 31) == 0) {
+            warp_sum[tid / 32] = make_float2(s, s2);
+        }
+    }
+    __syncthreads();
+    if (t.lanes > 32) {
+        if (tid < t.groups) {
+            float s = 0.0f, s2 = 0.0f;
+            for (uint32_t w = 0; w < t.lanes / 32; ++w) {
+                const float2 v = warp_sum[tid * (t.lanes / 32) + w];
+                s += v.x;
+                s2 += v.y;
+            }
+            sum[tid] = make_float2(s, s2);
+        }
+        __syncthreads();
+    }
+}
+
+// Group of the channel j places after c, relative to the tile's first.
+template <int L>
+__device__ __forceinline__ uint32_t channel_at(const Args& a, uint32_t c, int j) {
+    uint32_t ch = c + j;
+    if (L > 1) while (ch >= a.c) ch -= a.c;  // rows of several pixels
+    return ch;
+}
+
+// Large samples. Rows are whole block iterations, numbered over tiles, samples ("units") and rows. A block has
+// a run of them; a segment is its part of one unit.
+struct Run {
+    uint32_t w0, w1;
+};
+__device__ __forceinline__ Run run_of(const Args& a, const Plan& p, uint32_t b) {
+    if (p.per_unit) {
+        const uint32_t u = b / p.per_unit, r = (b - u * p.per_unit) * p.per_block;
+        return {u * p.rows + min(r, p.rows), u * p.rows + min(r + p.per_block, p.rows)};
+    }
+    const uint32_t total = p.rows * (uint32_t)a.n * p.tiles;
+    return {b * p.per_block, min((b + 1) * p.per_block, total)};
+}
+// Blocks whose runs meet unit u: [b0, b1].
+__device__ __forceinline__ void runs_of_unit(const Plan& p, uint32_t u, uint32_t& b0, uint32_t& b1) {
+    if (p.per_unit) {
+        b0 = u * p.per_unit;
+        b1 = b0 + p.per_unit - 1;
+    } else {
+        b0 = u * p.rows / p.per_block;
+        b1 = ((u + 1) * p.rows - 1) / p.per_block;
+    }
+}
+struct Segment {
+    uint32_t n, tile, c;  // sample, tile, channel of the thread's first element
+    uint32_t r0, iters, cnt;  // rows [r0, r0 + iters); cnt: of this thread, which misses at most a sample's last row
+    float pixels;
+};
+template <int V>
+__device__ __forceinline__ Segment segment_of(const Args& a, const Plan& p, uint32_t u, uint32_t from, uint32_t to,
+                                              const Tile& t) {
+    Segment s;
+    s.tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n;
+    s.n = u - s.tile * (uint32_t)a.n;
+    s.r0 = from - u * p.rows;
+    s.iters = to - from;
+    const uint32_t col = s.tile * p.cols + threadIdx.x;
+    const bool ends = s.r0 + s.iters == p.rows;
+    s.cnt = threadIdx.x < t.cols ? s.iters - (ends && col >= p.last) : 0;
+    s.c = col * V;
+    if (p.tiles == 1) s.c -= p.by_c(s.c) * a.c;
+    s.pixels = p.tiles > 1 ? (float)s.iters
+                           : (float)(uint64_t)(((uint64_t)(s.iters - ends) * p.rv + (ends ? p.last : 0)) * V / a.c);
+    return s;
+}
+// A thread's vector in a row, walked row by row through units.
+template <int V>
+struct Place {
+    uint64_t base;  // vectors before the thread's first one of this unit
+    uint32_t u, r;
+    bool in, in_last;
+
+    __device__ __forceinline__ void unit(const Args& a, const Plan& p) {
+        const uint32_t tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n, n = u - tile * (uint32_t)a.n;
+        const uint32_t col = tile * p.cols + threadIdx.x;
+        base = n * p.vecs + col;
+        in = threadIdx.x < p.cols && col < p.rv;
+        in_last = in && col < p.last;
+    }
+    __device__ __forceinline__ void start(const Args& a, const Plan& p, uint32_t w) {
+        u = w / p.rows;
+        r = w - u * p.rows;
+        unit(a, p);
+    }
+    __device__ __forceinline__ void next(const Args& a, const Plan& p) {
+        if (++r == p.rows) {
+            r = 0;
+            ++u;
+            unit(a, p);
+        }
+    }
+    __device__ __forceinline__ void before(const Args& a, const Plan& p) {
+        if (r-- == 0) {
+            r = p.rows - 1;
+            --u;
+            unit(a, p);
+        }
+    }
+    __device__ __forceinline__ bool valid(const Plan& p) const { return r + 1 == p.rows ? in_last : in; }
+    __device__ __forceinline__ uint64_t at(const Plan& p) const { return (base + (uint64_t)r * p.rv) * V; }
+};
+
+// Copies into a thread's own places of shared memory, which it alone reads: no barrier, only its own wait.
+template <class T, int V>
+__device__ __forceinline__ void copy_async(Pack<T, V>* to, const T* from) {
+    constexpr int bytes = V * (int)sizeof(T);
+    if constexpr (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+    else if constexpr (bytes >= 4)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(bytes) : "memory");
+    else
+        to->load(from);
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+// Joins what the runs of a unit left for its tile's groups: thread (l, q) takes group q of every lanes-th run,
+// f(slot) gives the value pair, and sum[q] holds the total for all threads.
+template <int V, class F>
+__device__ __forceinline__ void join_runs(const Args& a, const Plan& p, const Tile& t, uint32_t n,
+                                          float* part, float2* sum, F f) {
+    const uint32_t tid = threadIdx.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;
+    const uint32_t threads = blockDim.x;
+    for (uint32_t q0 = 0; q0 < t.groups; q0 += threads) {
+        const uint32_t groups = min(t.groups - q0, threads), each = threads / groups;
+        const uint32_t l = tid / groups, q = q0 + tid - l * groups;
+        float s = 0.0f, s2 = 0.0f;
+        if (l < each) {
+            const uint32_t grp = t.g0 + q;
+            const uint32_t t0 = p.tiles == 1 ? 0 : grp * a.per / tile_c;
+            const uint32_t t1 = p.tiles == 1 ? 0 : ((grp + 1) * a.per - 1) / tile_c;
+            for (uint32_t k = t0; k <= t1; ++k) {
+                const uint32_t u = k * (uint32_t)a.n + n, at = grp - (p.tiles == 1 ? 0 : p.by_per(k * tile_c));
+                uint32_t b0, b1;
+                runs_of_unit(p, u, b0, b1);
+#pragma unroll 4
+                for (uint32_t b = b0 + l; b <= b1; b += each) f((uint64_t)(b + u) * p.gl + at, q, s, s2);
+            }
+        }
+        part[tid] = s;
+        part[threads + tid] = s2;
+        __syncthreads();
+        uint32_t rows = each;  // of `groups` values: halved until few are left
+        while (rows > 4) {
+            const uint32_t half = (rows + 1) / 2;
+            if (l + half < rows) {
+                part[tid] += part[tid + half * groups];
+                part[threads + tid] += part[threads + tid + half * groups];
+            }
+            rows = half;
+            __syncthreads();
+        }
+        if (tid < groups) {
+            float r = 0.0f, r2 = 0.0f;
+            for (uint32_t m = 0; m < rows; ++m) {
+                r += part[m * groups + tid];
+                r2 += part[threads + m * groups + tid];
+            }
+            sum[q0 + tid] = make_float2(r, r2);
+        }
+        __syncthreads();
+    }
 }
 
 // Host side, one per element type (group_norm_{f32,bf16,f16}.cu). `whole`: a vector lies in one group.

@@ -8,36 +8,32 @@
 namespace bsx {
 namespace norm {
 
-// A thread's place in a tile and what it needs of its V channels.
+// What a thread needs of its V channels.
 template <class T, int V, int L>
 struct Lanes {
-    float a[V], b[V], mean[L];
+    float a[V], b[V], off[L];  // weight rstd, bias, -mean
 
-    __device__ __forceinline__ void params(const Args& g, uint32_t c) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const uint32_t ch = channel_at(g, c, j);
-            a[j] = param<T>(g.weight, g.param_f32, ch, 1.0f);
-            b[j] = param<T>(g.bias, g.param_f32, ch, 0.0f);
-        }
+    __device__ __forceinline__ void load(const Args& g, uint32_t c) {
+        params<T, V>(g, g.weight, c, L > 1, 1.0f, a);
+        params<T, V>(g, g.bias, c, L > 1, 0.0f, b);
     }
-    // stat[g]: mean and rstd
-    __device__ __forceinline__ void fold(const Args& g, const Tile& t, uint32_t c, const float2* stat) {
+    // stat[q]: mean and rstd of the tile's group q
+    __device__ __forceinline__ void fold(const Args& g, const Plan& p, const Tile& t, uint32_t c, const float2* stat) {
+        float r[L];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if (j < L || L > 1) {
-                const float2 s = stat[group_at<V, L>(g, t, c, j)];
-                mean[j] = s.x;
-                a[j] *= s.y;
-            } else {
-                a[j] *= stat[group_at<V, L>(g, t, c, 0)].y;
-            }
+        for (int j = 0; j < L; ++j) {
+            const float2 s = stat[p.by_per(channel_at<L>(g, c, j)) - t.g0];
+            off[j] = -s.x;
+            r[j] = s.y;
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) a[j] *= r[L > 1 ? j : 0];
     }
     template <int ACT>
     __device__ __forceinline__ void apply(float (&v)[V]) const {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = act<ACT>(__fmaf_rn(v[j] - mean[L > 1 ? j : 0], a[j], b[j]));
+        add_v<V>(v, v, off);  // exact for values near the mean: a large mean costs no digits
+        fma_v<V>(v, v, a, b);
+        activate<ACT>(v);
     }
 };
 
@@ -46,65 +42,67 @@ struct Lanes {
 template <class T, int V, int L, int ACT, bool DROP>
 __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
-    const Scratch<L, false> s(smem, p.gl);
-    const uint32_t tid = threadIdx.x, tile = blockIdx.x % p.tiles;
-    const uint64_t n = blockIdx.x / p.tiles;
+    float2* sum = (float2*)smem;           // [gl]
+    float2* warp_sum = sum + p.gl;         // [warps]
+    float* means = (float*)(warp_sum + kThreads / 32);  // [gl]
+    float* part = means + p.gl;            // [threads][L]
+    const uint32_t tid = threadIdx.x;
+    const uint32_t n = p.tiles == 1 ? blockIdx.x : blockIdx.x / p.tiles, tile = blockIdx.x - n * p.tiles;
     const Tile t = tile_of<V, L>(a, p, tile);
-    const uint32_t row = tid / t.cols, col = tile * p.cols + tid - row * t.cols;
+    const uint32_t row = t.cols == p.cols ? p.by_cols(tid) : tid / t.cols, col = tile * p.cols + tid - row * t.cols;
     const bool active = row < p.k;
-    const uint32_t rows = (uint32_t)p.rows - ((p.rows - 1) * p.rv + col >= p.vecs);  // of this column
-    const uint32_t cnt = active && row < rows ? (rows - row + p.k - 1) / p.k : 0;
-    const uint64_t at = (n * p.vecs + (uint64_t)row * p.rv + col) * V;
+    const uint32_t rows = p.rows - (col >= p.last);  // of this column
     const uint32_t step = p.k * p.rv * V;
+    const uint64_t at = (n * p.vecs + row * p.rv + col) * V;
     const T* x = (const T*)a.x + at;
     Pack<T, V> raw[kBatch];
+    uint32_t cnt = 0;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-        if (i < cnt) raw[i].load(x + (uint64_t)i * step);
-    const uint32_t c = col * V % a.c;
+        if (active && row + i * p.k < rows) {
+            raw[i].load(x + (uint64_t)i * step);
+            cnt = i + 1;
+        }
+    const uint32_t c = p.tiles > 1 ? col * V : col * V - p.by_c(col * V) * a.c;
     Lanes<T, V, L> lanes;
-    if (active) lanes.params(a, c);
+    if (active) lanes.load(a, c);
 
-    const float m = (float)(p.vecs * V / a.groups);  // values of a group
-    float sum[L] = {};
+    constexpr int P = kParts<V, L>;
+    const float m = (float)(a.pixels * a.per);  // values of a group
+    float acc[P] = {}, val[L], off[L];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
         if (i < cnt) {
             float f[V];
             raw[i].get(f);
-#pragma unroll
-            for (int j = 0; j < V; ++j) sum[L > 1 ? j : 0] += f[j];
+            accumulate<V, P>(acc, f);
         }
-    group_sums<V, L, false>(a, t, sum, sum, active, s.part, s.warp_sum, s.sum);
-    float mean[L];
+    per_item<V, L>(acc, val);
+    group_sums<V, L, false>(a, t, val, val, active, part, warp_sum, sum);
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-        mean[j] = active ? s.sum[group_at<V, L>(a, t, c, j)].x / m : 0.0f;
-        sum[j] = 0.0f;
-    }
+    for (int j = 0; j < L; ++j) off[j] = active ? -sum[p.by_per(channel_at<L>(a, c, j)) - t.g0].x / m : 0.0f;
+    for (uint32_t q = tid; q < t.groups; q += blockDim.x) means[q] = sum[q].x / m;
+#pragma unroll
+    for (int j = 0; j < P; ++j) acc[j] = 0.0f;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
         if (i < cnt) {
             float f[V];
             raw[i].get(f);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = f[j] - mean[L > 1 ? j : 0];
-                sum[L > 1 ? j : 0] = __fmaf_rn(d, d, sum[L > 1 ? j : 0]);
-            }
+            add_v<V>(f, f, off);
+            accumulate<V, P>(acc, f, f);
         }
-    float* means = s.end;  // [gl]: s.sum is filled again
-    for (uint32_t g = tid; g < t.groups; g += blockDim.x) means[g] = s.sum[g].x / m;
-    group_sums<V, L, false>(a, t, sum, sum, active, s.part, s.warp_sum, s.sum);
-    for (uint32_t g = tid; g < t.groups; g += blockDim.x) {
-        const float rstd = 1.0f / sqrtf(s.sum[g].x / m + a.eps);
-        s.sum[g] = make_float2(means[g], rstd);
-        a.mean[n * a.groups + t.g0 + g] = means[g];
-        a.rstd[n * a.groups + t.g0 + g] = rstd;
+    per_item<V, L>(acc, val);
+    group_sums<V, L, false>(a, t, val, val, active, part, warp_sum, sum);
+    for (uint32_t q = tid; q < t.groups; q += blockDim.x) {
+        const float rstd = 1.0f / sqrtf(sum[q].x / m + a.eps);
+        sum[q] = make_float2(means[q], rstd);
+        a.mean[(uint64_t)n * a.groups + t.g0 + q] = means[q];
+        a.rstd[(uint64_t)n * a.groups + t.g0 + q] = rstd;
     }
     __syncthreads();
     if (cnt == 0) return;
-    lanes.fold(a, t, c, s.sum);
+    lanes.fold(a, p, t, c, sum);
     const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
     T* out = (T*)a.out + at;
 #pragma unroll
@@ -119,189 +117,181 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
         }
 }
 
-// Large samples: one cooperative launch. The rows of all samples, tile after tile, are dealt to the blocks in
-// runs of per_block. First pass: mean and sum of squared deviations of each group in each run (from a pivot,
-// the mean of a thread's first vectors, so that no large mean cancels), to the workspace. Grid barrier. Second
-// pass, last row first: the runs' statistics are joined, and the rows are normalised from shared memory where
-// the first pass left its last `keep` iterations, and else from where they are nearest, L2 if they were read late.
+// Large samples: one cooperative launch, each block with a run of rows. Every thread copies its vector of the
+// coming rows into its own places of a ring in shared memory, kFlight rows ahead. First pass: mean and sum of
+// squared deviations of each group in each segment (from a pivot, the mean of a thread's first vectors, so that no
+// large mean cancels), to the workspace. Grid barrier. Second pass, last row first: the segments' statistics are
+// joined, and the rows are normalised out of the ring, which still holds the last ones; the others come again from
+// where they are nearest, L2 if they were read late.
 template <class T, int V, int L, int ACT, bool DROP>
 __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
-    const Scratch<L, false> s(smem, p.gl);
-    Pack<T, V>* kept = (Pack<T, V>*)(((uintptr_t)s.end + 15) & ~(uintptr_t)15);  // [keep][threads]
-    const uint32_t tid = threadIdx.x, step = p.k * p.rv * V;
-    const uint64_t total = p.rows * a.n * p.tiles, w0 = blockIdx.x * p.per_block;
-    const uint64_t w1 = w0 + p.per_block < total ? w0 + p.per_block : total;
-    const uint32_t all = run_iters(p, w0, w1);
-    const uint32_t kept_from = all > p.keep ? all - p.keep : 0;
+    float2* sum = (float2*)smem;                       // [gl]
+    float2* warp_sum = sum + p.gl;                     // [warps]
+    float2* pivot = warp_sum + kThreads / 32;          // [gl]
+    float* part = (float*)(pivot + p.gl);              // [threads][max(L, 2)]
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + blockDim.x * (L > 2 ? L : 2)) + 15) & ~(uintptr_t)15) + threadIdx.x;  // [ring][threads]
+    constexpr int P = kParts<V, L>, F = kFlight;
+    const uint32_t tid = threadIdx.x, threads = blockDim.x;
+    const Run run = run_of(a, p, blockIdx.x);
+    const uint32_t all = run.w1 - run.w0;
     float4* slots = (float4*)a.ws;  // [(block + unit) gl + group]: mean, squared deviations, count
 
-    uint32_t it = 0;
-    for (uint64_t w = w0; w < w1;) {
-        const uint64_t u = w / p.rows, to = (u + 1) * p.rows < w1 ? (u + 1) * p.rows : w1;
-        Tile t;
-        const Segment g = segment_of<V, L>(a, p, u, w, to, t);
-        const T* x = (const T*)a.x + g.at;
-        float pivot[L] = {}, sum[L] = {}, sq[L] = {};
-        Pack<T, V> cur[kFlight], nxt[kFlight];
-#pragma unroll
-        for (int i = 0; i < kFlight; ++i)
-            if (i < g.cnt) cur[i].load(x + (uint64_t)i * step);
-        for (uint32_t i0 = 0; i0 < g.iters; i0 += kFlight) {
-#pragma unroll
-            for (int i = 0; i < kFlight; ++i)
-                if (i0 + kFlight + i < g.cnt) nxt[i].load(x + (uint64_t)(i0 + kFlight + i) * step);
-            if (i0 == 0 && g.cnt) {
-                const uint32_t have = g.cnt < kFlight ? g.cnt : kFlight;
-#pragma unroll
-                for (int i = 0; i < kFlight; ++i)
-                    if (i < have) {
-                        float f[V];
-                        cur[i].get(f);
-#pragma unroll
-                        for (int j = 0; j < V; ++j) pivot[L > 1 ? j : 0] += f[j];
-                    }
-                const float inv = 1.0f / (float)(have * (V / L));
-#pragma unroll
-                for (int j = 0; j < L; ++j) pivot[j] *= inv;
+    Place<V> ahead;
+    ahead.start(a, p, run.w0);
+    uint32_t to_slot = 0, slot = 0;  // ring places of the row to copy and of the row at work
+    const auto copy = [&]() {
+        if (ahead.valid(p)) copy_async<T, V>(ring + to_slot * threads, (const T*)a.x + ahead.at(p));
+    };
+#pragma unroll 1
+    for (uint32_t i = 0; i < F; ++i) {
+        if (i < all) {
+            copy();
+            ahead.next(a, p);
+            to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
+        }
+        copy_commit();
+    }
+    for (uint32_t w = run.w0; w < run.w1;) {
+        const uint32_t u = w / p.rows, to = min((u + 1) * p.rows, run.w1);
+        const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
+        const Segment g = segment_of<V>(a, p, u, w, to, t);
+        float off[L] = {}, acc[P] = {}, sq[P] = {};
+        copy_wait<F - 4>();
+        if (g.cnt) {
+            const uint32_t have = min(g.cnt, 4u);
+            for (uint32_t i = 0, k = slot; i < have; ++i) {
+                float f[V];
+                ring[k * threads].get(f);
+                accumulate<V, P>(acc, f);
+                k = k + 1 == p.ring ? 0 : k + 1;
             }
+            per_item<V, L>(acc, off);
+            const float inv = -1.0f / (float)(have * (V / L));
 #pragma unroll
-            for (int i = 0; i < kFlight; ++i)
-                if (i0 + i < g.cnt) {
-                    float f[V];
-                    cur[i].get(f);
+            for (int j = 0; j < L; ++j) off[j] *= inv;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const int l = L > 1 ? j : 0;
-                        const float d = f[j] - pivot[l];
-                        sum[l] += d;
-                        sq[l] = __fmaf_rn(d, d, sq[l]);
-                    }
-                    if (it + i0 + i >= kept_from) kept[(it + i0 + i - kept_from) * blockDim.x + tid] = cur[i];
-                }
-#pragma unroll
-            for (int i = 0; i < kFlight; ++i) cur[i] = nxt[i];
+            for (int j = 0; j < P; ++j) acc[j] = 0.0f;
+        }
+#pragma unroll 2
+        for (uint32_t i = 0; i < g.iters; ++i, ++w) {
+            copy_wait<F - 1>();
+            if (i < g.cnt) {
+                float f[V];
+                ring[slot * threads].get(f);
+                add_v<V>(f, f, off);
+                accumulate<V, P>(acc, f);
+                accumulate<V, P>(sq, f, f);
+            }
+            slot = slot + 1 == p.ring ? 0 : slot + 1;
+            if (w + F < run.w1) {
+                copy();
+                ahead.next(a, p);
+                to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
+            }
+            copy_commit();
         }
         const float cnt = (float)g.cnt * (V / L);
-        float mean[L], dev[L], val[L];
+        float mean[L], dev[L], val[L], s[L], s2[L];
+        per_item<V, L>(acc, s);
+        per_item<V, L>(sq, s2);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const float d = g.cnt ? sum[j] / cnt : 0.0f;
-            mean[j] = pivot[j] + d;
-            dev[j] = __fmaf_rn(-sum[j], d, sq[j]);
-            if (dev[j] < 0.0f) dev[j] = 0.0f;
+            const float d = g.cnt ? s[j] / cnt : 0.0f;
+            mean[j] = d - off[j];
+            dev[j] = __fmaf_rn(-s[j], d, s2[j]);
+            if (dev[j] < 0.0f) dev[j] = 0.0f;  // rounding; NaN stays
             val[j] = cnt * mean[j];
         }
-        group_sums<V, L, false>(a, t, val, val, g.cnt != 0, s.part, s.warp_sum, s.sum);
-        float gm[L];
+        group_sums<V, L, false>(a, t, val, val, g.cnt != 0, part, warp_sum, sum);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            gm[j] = 0.0f;
+            val[j] = 0.0f;
             if (g.cnt) {
-                const uint32_t q = group_at<V, L>(a, t, g.c, j);
-                const uint32_t width = min((t.g0 + q + 1) * a.per, t.c1) - max((t.g0 + q) * a.per, t.c0);
-                gm[j] = s.sum[q].x / ((float)g.pixels * (float)width);
+                const uint32_t q = p.by_per(channel_at<L>(a, g.c, j)) - t.g0;
+                uint32_t lo, hi;
+                group_span<V, V>(a, t, q, lo, hi);
+                const float d = mean[j] - sum[q].x / (g.pixels * (float)(hi - lo));
+                val[j] = __fmaf_rn(cnt * d, d, dev[j]);
             }
-            const float d = mean[j] - gm[j];
-            val[j] = __fmaf_rn(cnt * d, d, dev[j]);
         }
-        float4* slot = slots + (blockIdx.x + u) * p.gl;
-        for (uint32_t q = tid; q < t.groups; q += blockDim.x) {
-            const uint32_t width = min((t.g0 + q + 1) * a.per, t.c1) - max((t.g0 + q) * a.per, t.c0);
-            const float count = (float)g.pixels * (float)width;
-            slot[q] = make_float4(s.sum[q].x / count, 0.0f, count, 0.0f);
+        float4* to_slots = slots + (uint64_t)(blockIdx.x + u) * p.gl;
+        for (uint32_t q = tid; q < t.groups; q += threads) {
+            uint32_t lo, hi;
+            group_span<V, V>(a, t, q, lo, hi);
+            const float count = g.pixels * (float)(hi - lo);
+            pivot[q] = make_float2(sum[q].x / count, count);
         }
-        group_sums<V, L, false>(a, t, val, val, g.cnt != 0, s.part, s.warp_sum, s.sum);
-        for (uint32_t q = tid; q < t.groups; q += blockDim.x) slot[q].y = s.sum[q].x;
-        it += g.iters;
-        w = to;
+        group_sums<V, L, false>(a, t, val, val, g.cnt != 0, part, warp_sum, sum);
+        for (uint32_t q = tid; q < t.groups; q += threads)
+            to_slots[q] = make_float4(pivot[q].x, sum[q].x, pivot[q].y, 0.0f);
     }
 
     cooperative_groups::this_grid().sync();
 
     const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
-    const uint32_t lane = tid & 31, warp = tid >> 5;
-    for (uint64_t end = w1; end > w0;) {
-        const uint64_t u = (end - 1) / p.rows, from = u * p.rows > w0 ? u * p.rows : w0;
-        Tile t;
-        const Segment g = segment_of<V, L>(a, p, u, from, end, t);
+    const float m = (float)(a.pixels * a.per);
+    const uint32_t resident = all > p.ring ? all - p.ring : 0;  // rows of the run from here on are in the ring
+    if (resident) ahead.start(a, p, run.w0 + resident - 1);
+    Place<V> here;
+    if (all) here.start(a, p, run.w1 - 1);
+    slot = all ? (all - 1) % p.ring : 0;
+    to_slot = resident ? (resident - 1) % p.ring : 0;
+    for (uint32_t end = run.w1; end > run.w0;) {
+        const uint32_t u = (end - 1) / p.rows, from = max(u * p.rows, run.w0);
+        const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
+        const Segment g = segment_of<V>(a, p, u, from, end, t);
         Lanes<T, V, L> lanes;
-        if (g.cnt) lanes.params(a, g.c);
-        __syncthreads();  // s.sum of the segment before is read no more
-        for (uint32_t q = warp; q < t.groups; q += blockDim.x / 32) {
+        if (g.cnt) lanes.load(a, g.c);
+        // Joined about a pivot, the mean of the unit's first segment: its share of the values bounds how far off it is.
+        uint32_t b0, b1;
+        runs_of_unit(p, u, b0, b1);
+        __syncthreads();  // sum and pivot are read no more
+        for (uint32_t q = tid; q < t.groups; q += threads) pivot[q].x = __ldcg(slots + (uint64_t)(b0 + u) * p.gl + q).x;
+        __syncthreads();
+        join_runs<V>(a, p, t, g.n, part, sum, [&](uint64_t i, uint32_t q, float& s, float& s2) {
+            const float4 v = __ldcg(slots + i);
+            const float d = v.x - pivot[q].x;
+            s = __fmaf_rn(v.z, d, s);
+            s2 += __fmaf_rn(v.z * d, d, v.y);
+        });
+        for (uint32_t q = tid; q < t.groups; q += threads) {
             const uint32_t grp = t.g0 + q;
-            const uint32_t tile_c = p.tiles == 1 ? a.c : p.cols * V;
-            const uint32_t t0 = grp * a.per / tile_c, t1 = ((grp + 1) * a.per - 1) / tile_c;
-            float sum = 0.0f, count = 0.0f;
-            for (uint32_t k = t0; k <= t1; ++k) {
-                const uint64_t uu = k * a.n + g.n;
-                const uint64_t b0 = uu * p.rows / p.per_block, b1 = ((uu + 1) * p.rows - 1) / p.per_block;
-                const uint32_t at = grp - k * tile_c / a.per;
-                for (uint64_t b = b0 + lane; b <= b1; b += 32) {
-                    const float4 v = __ldcg(slots + (b + uu) * p.gl + at);
-                    sum = __fmaf_rn(v.x, v.z, sum);
-                    count += v.z;
-                }
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                sum += __shfl_xor_sync(~0u, sum, o);
-                count += __shfl_xor_sync(~0u, count, o);
-            }
-            const float mean = sum / count;
-            float dev = 0.0f;
-            for (uint32_t k = t0; k <= t1; ++k) {
-                const uint64_t uu = k * a.n + g.n;
-                const uint64_t b0 = uu * p.rows / p.per_block, b1 = ((uu + 1) * p.rows - 1) / p.per_block;
-                const uint32_t at = grp - k * tile_c / a.per;
-                for (uint64_t b = b0 + lane; b <= b1; b += 32) {
-                    const float4 v = __ldcg(slots + (b + uu) * p.gl + at);
-                    const float d = v.x - mean;
-                    dev += __fmaf_rn(v.z * d, d, v.y);
-                }
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) dev += __shfl_xor_sync(~0u, dev, o);
-            const float rstd = 1.0f / sqrtf(dev / count + a.eps);
-            if (lane == 0) {
-                s.sum[q] = make_float2(mean, rstd);
-                if (g.r0 == 0 && grp * a.per >= t.c0) {
-                    a.mean[g.n * a.groups + grp] = mean;
-                    a.rstd[g.n * a.groups + grp] = rstd;
-                }
+            const float d = sum[q].x / m, mean = pivot[q].x + d;
+            float dev = __fmaf_rn(-sum[q].x, d, sum[q].y);
+            if (dev < 0.0f) dev = 0.0f;
+            const float rstd = 1.0f / sqrtf(dev / m + a.eps);
+            sum[q] = make_float2(mean, rstd);
+            if (g.r0 == 0 && grp * a.per >= t.c0) {
+                a.mean[(uint64_t)g.n * a.groups + grp] = mean;
+                a.rstd[(uint64_t)g.n * a.groups + grp] = rstd;
             }
         }
         __syncthreads();
-        it -= g.iters;
-        if (g.cnt) {
-            lanes.fold(a, t, g.c, s.sum);
-            const T* x = (const T*)a.x + g.at;
-            T* out = (T*)a.out + g.at;
-            for (uint32_t i1 = (g.cnt + kFlight - 1) / kFlight * kFlight; i1 > 0; i1 -= kFlight) {
-                Pack<T, V> raw[kFlight];
-#pragma unroll
-                for (int i = kFlight - 1; i >= 0; --i) {
-                    const uint32_t k = i1 - kFlight + i;
-                    if (k < g.cnt) {
-                        if (it + k >= kept_from) raw[i] = kept[(it + k - kept_from) * blockDim.x + tid];
-                        else raw[i].load(x + (uint64_t)k * step);
-                    }
-                }
-#pragma unroll
-                for (int i = kFlight - 1; i >= 0; --i) {
-                    const uint32_t k = i1 - kFlight + i;
-                    if (k < g.cnt) {
-                        float f[V];
-                        raw[i].get(f);
-                        lanes.template apply<ACT>(f);
-                        if (DROP) drop_vector<V>(a.drop, dstep, g.at + (uint64_t)k * step, f);
-                        raw[i].set(f);
-                        raw[i].store(out + (uint64_t)k * step);
-                    }
-                }
+        if (g.cnt) lanes.fold(a, p, t, g.c, sum);
+#pragma unroll 2
+        for (uint32_t i = g.iters; i-- > 0;) {
+            --end;
+            copy_wait<F - 1>();
+            if (i < g.cnt) {
+                float f[V];
+                ring[slot * threads].get(f);
+                lanes.template apply<ACT>(f);
+                const uint64_t at = here.at(p);
+                if (DROP) drop_vector<V>(a.drop, dstep, at, f);
+                Pack<T, V> o;
+                o.set(f);
+                o.store((T*)a.out + at);
             }
+            slot = slot == 0 ? p.ring - 1 : slot - 1;
+            if (end != run.w0) here.before(a, p);
+            if (end - run.w0 >= F && end - run.w0 - F < resident) {  // the row F places before
+                copy();
+                if (end - run.w0 > F) ahead.before(a, p);
+                to_slot = to_slot == 0 ? p.ring - 1 : to_slot - 1;
+            }
+            copy_commit();
         }
-        end = from;
     }
 }
 

@@ -46,50 +46,56 @@ template <class T, int V, int L, int ACT, bool DROP>
 cudaError_t launch_one(const Call& c) {
     const Args& a = *c.a;
     Plan& p = *c.p;
-    static std::atomic<uint64_t> done_small{0}, done_large{0};
     const int sms = sm_count(c.device);
-    if (p.small) {
-        if (!c.bwd) {
-            const uint32_t bytes = (sums_floats(p.threads, L, p.gl, false) + p.gl) * 4;
-            auto k = small_fwd_kernel<T, V, L, ACT, DROP>;
-            if (cudaError_t e = prepare(k, done_small, c.device)) return e;
-            k<<<p.blocks, p.threads, bytes, c.stream>>>(a, p);
-            return cudaSuccess;
-        }
-        const uint32_t bytes = sums_floats(p.threads, V, p.gl, true) * 4;
-        auto k = small_bwd_kernel<T, V, L, ACT, DROP>;
+    const uint32_t sums = 8 * (p.gl + kThreads / 32);  // sum, warp_sum
+    if (p.small && !c.bwd) {
         static std::atomic<uint64_t> done{0};
+        auto k = small_fwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
+        k<<<p.blocks, p.threads, sums + 4 * (p.gl + p.threads * L), c.stream>>>(a, p);
+        return cudaSuccess;
+    }
+    if (p.small) {
+        static std::atomic<uint64_t> done{0};
+        auto k = small_bwd_kernel<T, V, L, ACT, DROP>;
+        if (cudaError_t e = prepare(k, done, c.device)) return e;
+        const uint32_t bytes = sums + 8 * p.threads * V;
         int per_sm = 1;
-        if (p.blocks > (uint32_t)sms) {
+        if (p.blocks > (uint32_t)sms)
             if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, (int)p.threads, bytes)) return e;
-        }
-        uint32_t most = (uint32_t)(sms * per_sm);
-        if (most > kMaxBlocks) most = kMaxBlocks;
-        uint32_t blocks = p.blocks < most ? p.blocks : most / p.tiles * p.tiles;
+        const uint32_t most = (uint32_t)(sms * per_sm) < kMaxBlocks ? (uint32_t)(sms * per_sm) : kMaxBlocks;
+        return cooperative(k, a, p, p.blocks < most ? p.blocks : most / p.tiles * p.tiles, bytes, c.stream);
+    }
+    const uint32_t tile_c = p.tiles == 1 ? a.c : p.cols * V;
+    const uint32_t head = c.bwd ? 8 * (p.gl + tile_c + p.threads * V) : sums + 8 * p.gl + 4 * p.threads * (L > 2 ? L : 2);
+    const uint32_t row = p.threads * (uint32_t)sizeof(Pack<T, V>) * (c.bwd ? 2 : 1);  // a single 16-bit element takes a word
+    // Runs: where units are few, each has blocks of its own, so that no block sums and joins twice; where that
+    // would leave more than a tenth of the SMs idle, runs cross units.
+    const uint32_t units = (uint32_t)a.n * p.tiles, total = p.rows * units;
+    uint32_t blocks = total < (uint32_t)sms ? total : (uint32_t)sms;
+    p.per_unit = blocks / units;
+    if (p.per_unit > 0 && p.per_unit * units * 10 >= blocks * 9) {
+        p.per_block = (p.rows + p.per_unit - 1) / p.per_unit;
+        p.per_unit = (p.rows + p.per_block - 1) / p.per_block;
+        blocks = p.per_unit * units;
+    } else {
+        p.per_unit = 0;
+        p.per_block = (total + blocks - 1) / blocks;
+        blocks = (total + p.per_block - 1) / p.per_block;
+    }
+    p.ring = (kSharedMost - 16 - head) / row;
+    if (p.ring > p.per_block) p.ring = p.per_block;
+    const uint32_t bytes = head + 16 + p.ring * row;
+    if (c.bwd) {
+        static std::atomic<uint64_t> done{0};
+        auto k = large_bwd_kernel<T, V, L, ACT, DROP>;
+        if (cudaError_t e = prepare(k, done, c.device)) return e;
         return cooperative(k, a, p, blocks, bytes, c.stream);
     }
-    const uint32_t head = (sums_floats(p.threads, c.bwd ? V : L, p.gl, c.bwd) * 4 + 15) / 16 * 16;
-    const uint32_t slot = p.threads * (uint32_t)sizeof(Pack<T, V>) * (c.bwd ? 2 : 1);  // a single 16-bit element takes a word
-    p.keep = (kSharedMost - 16 - head) / slot;
-    const uint64_t total = p.rows * a.n * p.tiles;
-    uint64_t blocks = (total + p.k - 1) / p.k;
-    if (blocks > (uint64_t)sms) blocks = sms;
-    p.per_block = ((total + blocks - 1) / blocks + p.k - 1) / p.k * p.k;
-    blocks = (total + p.per_block - 1) / p.per_block;
-    // no more shared memory than the longest run can use
-    const uint64_t iters = (p.per_block + p.k - 1) / p.k + p.per_block / p.rows + 2;
-    if (p.keep > iters) p.keep = (uint32_t)iters;
-    const uint32_t bytes = head + 16 + p.keep * slot;
-    if (c.bwd) {
-        auto k = large_bwd_kernel<T, V, L, ACT, DROP>;
-        static std::atomic<uint64_t> done{0};
-        if (cudaError_t e = prepare(k, done, c.device)) return e;
-        return cooperative(k, a, p, (uint32_t)blocks, bytes, c.stream);
-    }
+    static std::atomic<uint64_t> done{0};
     auto k = large_fwd_kernel<T, V, L, ACT, DROP>;
-    if (cudaError_t e = prepare(k, done_large, c.device)) return e;
-    return cooperative(k, a, p, (uint32_t)blocks, bytes, c.stream);
+    if (cudaError_t e = prepare(k, done, c.device)) return e;
+    return cooperative(k, a, p, blocks, bytes, c.stream);
 }
 
 template <class T, int V, int L>
