@@ -17,9 +17,9 @@ namespace norm {
 
 constexpr int kThreads = 512;         // most threads of a block
 constexpr int kBatch = 8;             // vectors a thread holds, small samples
-constexpr int kFlight = 8;            // rows in flight ahead of the one at work, large samples
-constexpr int kBatchBwd = 4;          // the same two for the backward, of x and of v each
-constexpr int kFlightBwd = 5;
+constexpr int kRows = 4, kAhead = 2;  // large samples: rows of a batch, batches in flight ahead of the one at work
+constexpr int kBatchBwd = 4;          // the same for the backward, of x and of v each
+constexpr int kRowsBwd = 2, kAheadBwd = 2;
 constexpr uint32_t kMaxBlocks = 512;  // most blocks of a kernel that leaves partial sums
 
 // Division of x by d for x d < 2^32: with f = (2^32 + e) / d, 0 < e <= d, the product's high word is
@@ -62,7 +62,7 @@ struct Plan {
     uint32_t gl;         // most groups of a tile
     uint32_t per_block;  // large samples: rows of a block
     uint32_t per_unit;   // blocks of a (tile, sample); 0: the rows of all of them are dealt to the blocks in order
-    uint32_t ring;       // rows in shared memory
+    uint32_t ring;       // batches in shared memory
     uint32_t threads, blocks;
     uint32_t v;          // elements of a vector
     int small;           // one block per (sample, tile), everything in registers
@@ -176,7 +176,7 @@ __device__ __forceinline__ void per_item(const float (&part)[kParts<V, L>], floa
     }
 }
 
-// The approximate exponential and reciprocal (2 and 1 ulp); results below 2^-126 become 0.
+// The approximate exponential and reciprocal (2 and 1 ulp).
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -189,50 +189,61 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 
 // act(z) = z s(w(z)), s the logistic function: w = z (silu), or 2 sqrt(2/pi) (z + 0.044715 z^3)
-// (gelu in its tanh form, because (1 + tanh(t)) / 2 = s(2 t)). s = 1 / (1 + 2^(-w log2 e)); both
-// ends are right: the exponential overflows to infinity and s is 0, or it vanishes and s is 1.
+// (gelu in its tanh form, because (1 + tanh(t)) / 2 = s(2 t)). With e = 2^(-w log2 e) it is
+// s = 1 / (1 + e). The special-function unit takes eight cycles for an exponential or reciprocal
+// of a warp and would bound a pass over 16-bit data, so two reciprocals are one of the product:
+// 1 / a = b / (a b). Exponents are held below 60 so that the product stays finite: s is right to
+// a few units in the last place above 2^-60, and 2^-60 below.
 constexpr float kLog2e = 1.4426950408889634f, kGelu1 = 1.5957691216057308f, kGelu3 = 0.044715f;
 template <int ACT, int V>
-__device__ __forceinline__ void gates(const float (&z)[V], float (&s)[V]) {
+__device__ __forceinline__ void gates(const float (&z)[V], float (&s)[V], float (&e)[V]) {
     constexpr float one[1] = {1.0f};
     if (ACT == BSX_ACT_SILU) {
         constexpr float k[1] = {-kLog2e};
-        mul_v<V>(s, z, k);
+        mul_v<V>(e, z, k);
     } else {
         constexpr float k1[1] = {-kLog2e * kGelu1}, k3[1] = {-kLog2e * kGelu1 * kGelu3};
-        mul_v<V>(s, z, z);
-        fma_v<V>(s, s, k3, k1);
-        mul_v<V>(s, s, z);
+        mul_v<V>(e, z, z);
+        fma_v<V>(e, e, k3, k1);
+        mul_v<V>(e, e, z);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = exp2_fast(s[j]);
-    add_v<V>(s, s, one);
+    for (int j = 0; j < V; ++j) e[j] = exp2_fast(fminf(e[j], 60.0f));
+    add_v<V>(s, e, one);
+    if constexpr (V == 1) {
+        s[0] = rcp_fast(s[0]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = rcp_fast(s[j]);
+        for (int j = 0; j < V; j += 2) {
+            const float r = rcp_fast(s[j] * s[j + 1]);
+            mul2(s[j], s[j + 1], s[j + 1], s[j], r, r);
+        }
+    }
 }
 template <int ACT, int V>
 __device__ __forceinline__ void activate(float (&z)[V]) {
     if constexpr (ACT != BSX_ACT_NONE) {
-        float s[V];
-        gates<ACT>(z, s);
+        float s[V], e[V];
+        gates<ACT>(z, s, e);
         mul_v<V>(z, z, s);
     }
 }
-// act'(z) = s + (s - s^2) z w'(z)
+// act'(z) = s + s (1 - s) z w'(z) = s (1 + e s z w'(z)): 1 - s = e s without a difference. NaN goes through z.
 template <int ACT, int V>
 __device__ __forceinline__ void slopes(float (&z)[V]) {
-    float s[V], t[V], neg[V];
-    gates<ACT>(z, s);
+    constexpr float one[1] = {1.0f};
+    float s[V], e[V];
+    gates<ACT>(z, s, e);
+    mul_v<V>(e, e, s);
     if (ACT == BSX_ACT_GELU_TANH) {
         constexpr float k1[1] = {kGelu1}, k3[1] = {3.0f * kGelu1 * kGelu3};
+        float t[V];
         mul_v<V>(t, z, z);
         fma_v<V>(t, t, k3, k1);
         mul_v<V>(z, z, t);
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) neg[j] = -s[j];
-    fma_v<V>(t, neg, s, s);
-    fma_v<V>(z, t, z, s);
+    fma_v<V>(z, e, z, one);
+    mul_v<V>(z, z, s);
 }
 
 // drop for V elements from flat element `at` (V divides it, and 8).
@@ -375,8 +386,9 @@ __device__ __forceinline__ void runs_of_unit(const Plan& p, uint32_t u, uint32_t
     }
 }
 struct Segment {
-    uint32_t n, tile, c;  // sample, tile, channel of the thread's first element
+    uint32_t n, tile, c;      // sample, tile, channel of the thread's first element
     uint32_t r0, iters, cnt;  // rows [r0, r0 + iters); cnt: of this thread, which misses at most a sample's last row
+    uint64_t at;              // first element of the thread's vector in row r0
     float pixels;
 };
 template <int V>
@@ -390,47 +402,58 @@ __device__ __forceinline__ Segment segment_of(const Args& a, const Plan& p, uint
     const uint32_t col = s.tile * p.cols + threadIdx.x;
     const bool ends = s.r0 + s.iters == p.rows;
     s.cnt = threadIdx.x < t.cols ? s.iters - (ends && col >= p.last) : 0;
+    s.at = (s.n * p.vecs + (uint64_t)s.r0 * p.rv + col) * V;
     s.c = col * V;
     if (p.tiles == 1) s.c -= p.by_c(s.c) * a.c;
     s.pixels = p.tiles > 1 ? (float)s.iters
                            : (float)(uint64_t)(((uint64_t)(s.iters - ends) * p.rv + (ends ? p.last : 0)) * V / a.c);
     return s;
 }
-// A thread's vector in a row, walked row by row through units.
-template <int V>
-struct Place {
-    uint64_t base;  // vectors before the thread's first one of this unit
-    uint32_t u, r;
-    bool in, in_last;
+// Batches of R rows of a run, each inside one segment, counted from the segment's first row.
+template <int R>
+__device__ __forceinline__ uint32_t batches_of(const Plan& p, const Run& run) {
+    uint32_t all = 0;
+    for (uint32_t w = run.w0; w < run.w1;) {
+        const uint32_t to = min((w / p.rows + 1) * p.rows, run.w1);
+        all += (to - w + R - 1) / R;
+        w = to;
+    }
+    return all;
+}
+// The batch that is copied next: a walk over a run's batches, forwards or backwards.
+template <int V, int R>
+struct Walk {
+    uint32_t u, w, from, to, valid;  // unit; first row; the segment; end of the rows in which the thread has a vector
+    uint64_t at;                     // element of row w
 
-    __device__ __forceinline__ void unit(const Args& a, const Plan& p) {
+    __device__ __forceinline__ void unit(const Args& a, const Plan& p, const Run& run, bool last) {
+        from = max(u * p.rows, run.w0);
+        to = min((u + 1) * p.rows, run.w1);
+        w = last ? from + (to - 1 - from) / R * R : from;
         const uint32_t tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n, n = u - tile * (uint32_t)a.n;
         const uint32_t col = tile * p.cols + threadIdx.x;
-        base = n * p.vecs + col;
-        in = threadIdx.x < p.cols && col < p.rv;
-        in_last = in && col < p.last;
+        valid = threadIdx.x < p.cols && col < p.rv ? to - (to == (u + 1) * p.rows && col >= p.last) : 0;
+        at = (n * p.vecs + (uint64_t)(w - u * p.rows) * p.rv + col) * V;
     }
-    __device__ __forceinline__ void start(const Args& a, const Plan& p, uint32_t w) {
-        u = w / p.rows;
-        r = w - u * p.rows;
-        unit(a, p);
-    }
-    __device__ __forceinline__ void next(const Args& a, const Plan& p) {
-        if (++r == p.rows) {
-            r = 0;
+    __device__ __forceinline__ void next(const Args& a, const Plan& p, const Run& run) {
+        w += R;
+        at += (uint64_t)(R * V) * p.rv;
+        if (w >= to && to < run.w1) {
             ++u;
-            unit(a, p);
+            unit(a, p, run, false);
         }
     }
-    __device__ __forceinline__ void before(const Args& a, const Plan& p) {
-        if (r-- == 0) {
-            r = p.rows - 1;
-            --u;
-            unit(a, p);
+    __device__ __forceinline__ void before(const Args& a, const Plan& p, const Run& run) {
+        if (w == from) {
+            if (from > run.w0) {
+                --u;
+                unit(a, p, run, true);
+            }
+        } else {
+            w -= R;
+            at -= (uint64_t)(R * V) * p.rv;
         }
     }
-    __device__ __forceinline__ bool valid(const Plan& p) const { return r + 1 == p.rows ? in_last : in; }
-    __device__ __forceinline__ uint64_t at(const Plan& p) const { return (base + (uint64_t)r * p.rv) * V; }
 };
 
 // Copies into a thread's own places of shared memory, which it alone reads: no barrier, only its own wait.

@@ -214,39 +214,44 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
 template <class T, int V, int L, int ACT, bool DROP>
 __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
-    constexpr int F = kFlightBwd;
+    constexpr int R = kRowsBwd, F = kAheadBwd;
     const uint32_t tid = threadIdx.x, threads = blockDim.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;
     float2* sum = (float2*)smem;            // [gl]
     float2* chan = sum + p.gl;              // [tile_c]
     float* part = (float*)(chan + tile_c);  // [2][threads][V]
-    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + threads * 2 * V) + 15) & ~(uintptr_t)15) + tid;  // [ring][x, v][threads]
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + threads * 2 * V) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][x, v][threads]
+    const uint64_t step = (uint64_t)p.rv * V;
     const Run run = run_of(a, p, blockIdx.x);
-    const uint32_t all = run.w1 - run.w0;
+    const uint32_t all = batches_of<R>(p, run);
     const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
     float2* slots = (float2*)a.ws;                                                   // [(block + unit) gl + group]
     float2* chans = slots + (uint64_t)(gridDim.x + p.tiles * (uint32_t)a.n) * p.gl;  // [(block + tile) tile_c + channel - c0]
     const bool wanted = a.v_weight || a.v_bias;
 
-    Place<V> ahead, here;
-    ahead.start(a, p, run.w0);
-    here.start(a, p, run.w0);
+    Walk<V, R> ahead;
+    ahead.u = run.w0 / p.rows;
+    ahead.unit(a, p, run, false);
     uint32_t to_slot = 0, slot = 0;
     const auto copy = [&]() {
-        if (ahead.valid(p)) {
-            const uint64_t at = ahead.at(p);
-            copy_async<T, V>(ring + 2 * to_slot * threads, (const T*)a.x + at);
-            copy_async<T, V>(ring + (2 * to_slot + 1) * threads, (const T*)a.v + at);
-        }
+        Pack<T, V>* to = ring + to_slot * 2 * R * threads;
+        const T *x = (const T*)a.x + ahead.at, *v = (const T*)a.v + ahead.at;
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+            if (ahead.w + j < ahead.valid) {
+                copy_async<T, V>(to + 2 * j * threads, x + j * step);
+                copy_async<T, V>(to + (2 * j + 1) * threads, v + j * step);
+            }
     };
 #pragma unroll 1
-    for (uint32_t i = 0; i < F; ++i) {
-        if (i < all) {
+    for (uint32_t b = 0; b < F; ++b) {
+        if (b < all) {
             copy();
-            ahead.next(a, p);
+            ahead.next(a, p, run);
             to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
         }
         copy_commit();
     }
+    uint32_t batch = 0;
     bool first = true;  // first segment of the block in its tile
     for (uint32_t w = run.w0; w < run.w1;) {
         const uint32_t u = w / p.rows, to = min((u + 1) * p.rows, run.w1);
@@ -258,23 +263,32 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             lanes.stats(a, p, g.n, g.c);
         }
         float sa[V] = {}, sb[V] = {};
-#pragma unroll 2
-        for (uint32_t i = 0; i < g.iters; ++i, ++w) {
+        uint64_t at = g.at;
+        const auto take = [&](const Pack<T, V>& px, const Pack<T, V>& pv, uint64_t where) {
+            float fx[V], fv[V];
+            px.get(fx);
+            pv.get(fv);
+            if (DROP) drop_vector<V>(a.drop, dstep, where, fv);
+            lanes.template grads<ACT>(fx, fv);
+            accumulate<V, V>(sa, fv);
+            accumulate<V, V>(sb, fv, fx);
+        };
+        for (uint32_t i0 = 0; i0 < g.iters; i0 += R, ++batch) {
             copy_wait<F - 1>();
-            if (i < g.cnt) {
-                float fx[V], fv[V];
-                ring[2 * slot * threads].get(fx);
-                ring[(2 * slot + 1) * threads].get(fv);
-                if (DROP) drop_vector<V>(a.drop, dstep, here.at(p), fv);
-                lanes.template grads<ACT>(fx, fv);
-                accumulate<V, V>(sa, fv);
-                accumulate<V, V>(sb, fv, fx);
+            const Pack<T, V>* have = ring + slot * 2 * R * threads;
+            if (i0 + R <= g.cnt) {
+#pragma unroll
+                for (int j = 0; j < R; ++j) take(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
+            } else {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    if (i0 + j < g.cnt) take(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
             }
+            at += R * step;
             slot = slot + 1 == p.ring ? 0 : slot + 1;
-            if (DROP) here.next(a, p);
-            if (w + F < run.w1) {
+            if (batch + F < all) {
                 copy();
-                ahead.next(a, p);
+                ahead.next(a, p, run);
                 to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
             }
             copy_commit();
@@ -317,17 +331,23 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             to_slots[q] = make_float2(s1, s2);
         }
         __syncthreads();
+        w = to;
         first = p.tiles > 1 && w / p.rows / (uint32_t)a.n != g.tile;
     }
 
     cooperative_groups::this_grid().sync();
 
     const float m = (float)(a.pixels * a.per);
-    const uint32_t resident = all > p.ring ? all - p.ring : 0;  // rows of the run from here on are in the ring
-    if (resident) ahead.start(a, p, run.w0 + resident - 1);
-    if (all) here.start(a, p, run.w1 - 1);
-    slot = all ? (all - 1) % p.ring : 0;
-    to_slot = resident ? (resident - 1) % p.ring : 0;
+    const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
+    uint32_t next = all - 1;                                    // the batch that `ahead` is at
+    ahead.u = (run.w1 - 1) / p.rows;
+    ahead.unit(a, p, run, true);
+    while (next >= resident && next > 0) {
+        ahead.before(a, p, run);
+        --next;
+    }
+    slot = (all - 1) % p.ring;
+    to_slot = next % p.ring;
     for (uint32_t end = run.w1; end > run.w0;) {
         const uint32_t u = (end - 1) / p.rows, from = max(u * p.rows, run.w0);
         const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
@@ -345,31 +365,44 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             s2 += v.y;
         });
         if (g.cnt) gg.take(a, p, t, g.c, sum, m, lanes);
-#pragma unroll 2
-        for (uint32_t i = g.iters; i-- > 0;) {
-            --end;
+        uint64_t at = g.at + (g.iters - 1) / R * R * step;
+        const auto give = [&](const Pack<T, V>& px, const Pack<T, V>& pv, uint64_t where) {
+            float fx[V], fv[V];
+            px.get(fx);
+            pv.get(fv);
+            if (DROP) drop_vector<V>(a.drop, dstep, where, fv);
+            lanes.template grads<ACT>(fx, fv);
+            gg.apply(fx, fv);
+            Pack<T, V> o;
+            o.set(fx);
+            o.store((T*)a.out + where);
+        };
+        for (uint32_t i0 = (g.iters - 1) / R * R;; i0 -= R) {
+            --batch;
             copy_wait<F - 1>();
-            if (i < g.cnt) {
-                float fx[V], fv[V];
-                ring[2 * slot * threads].get(fx);
-                ring[(2 * slot + 1) * threads].get(fv);
-                const uint64_t at = here.at(p);
-                if (DROP) drop_vector<V>(a.drop, dstep, at, fv);
-                lanes.template grads<ACT>(fx, fv);
-                gg.apply(fx, fv);
-                Pack<T, V> o;
-                o.set(fx);
-                o.store((T*)a.out + at);
+            const Pack<T, V>* have = ring + slot * 2 * R * threads;
+            if (i0 + R <= g.cnt) {
+#pragma unroll
+                for (int j = 0; j < R; ++j) give(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
+            } else {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    if (i0 + j < g.cnt) give(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
             }
+            at -= R * step;
             slot = slot == 0 ? p.ring - 1 : slot - 1;
-            if (end != run.w0) here.before(a, p);
-            if (end - run.w0 >= F && end - run.w0 - F < resident) {  // the row F places before
+            if (batch == next + F && next < resident) {
                 copy();
-                if (end - run.w0 > F) ahead.before(a, p);
                 to_slot = to_slot == 0 ? p.ring - 1 : to_slot - 1;
+                if (next > 0) {
+                    ahead.before(a, p, run);
+                    --next;
+                }
             }
             copy_commit();
+            if (i0 == 0) break;
         }
+        end = from;
     }
     if (wanted)
         for (uint32_t ch = blockIdx.x * (threads / 32) + tid / 32; ch < a.c; ch += gridDim.x * (threads / 32)) {

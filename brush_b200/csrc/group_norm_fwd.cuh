@@ -117,138 +117,160 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
         }
 }
 
-// Large samples: one cooperative launch, each block with a run of rows. Every thread copies its vector of the
-// coming rows into its own places of a ring in shared memory, kFlight rows ahead. First pass: mean and sum of
-// squared deviations of each group in each segment (from a pivot, the mean of a thread's first vectors, so that no
-// large mean cancels), to the workspace. Grid barrier. Second pass, last row first: the segments' statistics are
-// joined, and the rows are normalised out of the ring, which still holds the last ones; the others come again from
-// where they are nearest, L2 if they were read late.
+// Large samples: one cooperative launch, each block with a run of rows. Every thread copies its vectors of the
+// coming batches of rows into its own places of a ring in shared memory, kAhead batches ahead. First pass: mean and
+// sum of squared deviations of each group in each segment (from a pivot, the mean of a thread's first vectors, so
+// that no large mean cancels), to the workspace. Grid barrier. Second pass, last row first: the segments' statistics
+// are joined, and the rows are normalised out of the ring, which still holds the last ones; the others come again.
 template <class T, int V, int L, int ACT, bool DROP>
 __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;                       // [gl]
     float2* warp_sum = sum + p.gl;                     // [warps]
-    float2* pivot = warp_sum + kThreads / 32;          // [gl]
+    float2* pivot = warp_sum + kThreads / 32;          // [gl]: mean and count of the block's last segment
     float* part = (float*)(pivot + p.gl);              // [threads][max(L, 2)]
-    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + blockDim.x * (L > 2 ? L : 2)) + 15) & ~(uintptr_t)15) + threadIdx.x;  // [ring][threads]
-    constexpr int P = kParts<V, L>, F = kFlight;
     const uint32_t tid = threadIdx.x, threads = blockDim.x;
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + threads * (L > 2 ? L : 2)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][threads]
+    constexpr int P = kParts<V, L>, R = kRows, F = kAhead;
+    const uint64_t step = (uint64_t)p.rv * V;
     const Run run = run_of(a, p, blockIdx.x);
-    const uint32_t all = run.w1 - run.w0;
+    const uint32_t all = batches_of<R>(p, run);
     float4* slots = (float4*)a.ws;  // [(block + unit) gl + group]: mean, squared deviations, count
 
-    Place<V> ahead;
-    ahead.start(a, p, run.w0);
-    uint32_t to_slot = 0, slot = 0;  // ring places of the row to copy and of the row at work
+    Walk<V, R> ahead;
+    ahead.u = run.w0 / p.rows;
+    ahead.unit(a, p, run, false);
+    uint32_t to_slot = 0, slot = 0;  // ring places of the batch to copy and of the batch at work
     const auto copy = [&]() {
-        if (ahead.valid(p)) copy_async<T, V>(ring + to_slot * threads, (const T*)a.x + ahead.at(p));
+        Pack<T, V>* to = ring + to_slot * R * threads;
+        const T* x = (const T*)a.x + ahead.at;
+        if (ahead.w + R <= ahead.valid) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) copy_async<T, V>(to + j * threads, x + j * step);
+        } else {
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+                if (ahead.w + j < ahead.valid) copy_async<T, V>(to + j * threads, x + j * step);
+        }
     };
 #pragma unroll 1
-    for (uint32_t i = 0; i < F; ++i) {
-        if (i < all) {
+    for (uint32_t b = 0; b < F; ++b) {
+        if (b < all) {
             copy();
-            ahead.next(a, p);
+            ahead.next(a, p, run);
             to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
         }
         copy_commit();
     }
+    uint32_t batch = 0;
     for (uint32_t w = run.w0; w < run.w1;) {
         const uint32_t u = w / p.rows, to = min((u + 1) * p.rows, run.w1);
         const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
         const Segment g = segment_of<V>(a, p, u, w, to, t);
         float off[L] = {}, acc[P] = {}, sq[P] = {};
-        copy_wait<F - 4>();
-        if (g.cnt) {
-            const uint32_t have = min(g.cnt, 4u);
-            for (uint32_t i = 0, k = slot; i < have; ++i) {
-                float f[V];
-                ring[k * threads].get(f);
-                accumulate<V, P>(acc, f);
-                k = k + 1 == p.ring ? 0 : k + 1;
-            }
-            per_item<V, L>(acc, off);
-            const float inv = -1.0f / (float)(have * (V / L));
-#pragma unroll
-            for (int j = 0; j < L; ++j) off[j] *= inv;
-#pragma unroll
-            for (int j = 0; j < P; ++j) acc[j] = 0.0f;
-        }
-#pragma unroll 2
-        for (uint32_t i = 0; i < g.iters; ++i, ++w) {
+        const auto take = [&](const Pack<T, V>& v) {
+            float f[V];
+            v.get(f);
+            add_v<V>(f, f, off);
+            accumulate<V, P>(acc, f);
+            accumulate<V, P>(sq, f, f);
+        };
+        for (uint32_t i0 = 0; i0 < g.iters; i0 += R, ++batch) {
             copy_wait<F - 1>();
-            if (i < g.cnt) {
-                float f[V];
-                ring[slot * threads].get(f);
-                add_v<V>(f, f, off);
-                accumulate<V, P>(acc, f);
-                accumulate<V, P>(sq, f, f);
+            const Pack<T, V>* at = ring + slot * R * threads;
+            if (i0 == 0 && g.cnt) {
+                const uint32_t have = min(g.cnt, (uint32_t)R);
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    if (j < have) {
+                        float f[V];
+                        at[j * threads].get(f);
+                        accumulate<V, P>(acc, f);
+                    }
+                per_item<V, L>(acc, off);
+                const float inv = -1.0f / (float)(have * (V / L));
+#pragma unroll
+                for (int j = 0; j < L; ++j) off[j] *= inv;
+#pragma unroll
+                for (int j = 0; j < P; ++j) acc[j] = 0.0f;
+            }
+            if (i0 + R <= g.cnt) {
+#pragma unroll
+                for (int j = 0; j < R; ++j) take(at[j * threads]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    if (i0 + j < g.cnt) take(at[j * threads]);
             }
             slot = slot + 1 == p.ring ? 0 : slot + 1;
-            if (w + F < run.w1) {
+            if (batch + F < all) {
                 copy();
-                ahead.next(a, p);
+                ahead.next(a, p, run);
                 to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
             }
             copy_commit();
         }
-        const float cnt = (float)g.cnt * (V / L);
+        const float cnt = (float)g.cnt * (V / L), inv = g.cnt ? 1.0f / cnt : 0.0f;
         float mean[L], dev[L], val[L], s[L], s2[L];
         per_item<V, L>(acc, s);
         per_item<V, L>(sq, s2);
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const float d = g.cnt ? s[j] / cnt : 0.0f;
+            const float d = s[j] * inv;
             mean[j] = d - off[j];
             dev[j] = __fmaf_rn(-s[j], d, s2[j]);
             if (dev[j] < 0.0f) dev[j] = 0.0f;  // rounding; NaN stays
             val[j] = cnt * mean[j];
         }
         group_sums<V, L, false>(a, t, val, val, g.cnt != 0, part, warp_sum, sum);
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            val[j] = 0.0f;
-            if (g.cnt) {
-                const uint32_t q = p.by_per(channel_at<L>(a, g.c, j)) - t.g0;
-                uint32_t lo, hi;
-                group_span<V, V>(a, t, q, lo, hi);
-                const float d = mean[j] - sum[q].x / (g.pixels * (float)(hi - lo));
-                val[j] = __fmaf_rn(cnt * d, d, dev[j]);
-            }
-        }
-        float4* to_slots = slots + (uint64_t)(blockIdx.x + u) * p.gl;
         for (uint32_t q = tid; q < t.groups; q += threads) {
             uint32_t lo, hi;
             group_span<V, V>(a, t, q, lo, hi);
             const float count = g.pixels * (float)(hi - lo);
             pivot[q] = make_float2(sum[q].x / count, count);
         }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < L; ++j) {
+            val[j] = 0.0f;
+            if (g.cnt) {
+                const float d = mean[j] - pivot[p.by_per(channel_at<L>(a, g.c, j)) - t.g0].x;
+                val[j] = __fmaf_rn(cnt * d, d, dev[j]);
+            }
+        }
         group_sums<V, L, false>(a, t, val, val, g.cnt != 0, part, warp_sum, sum);
         for (uint32_t q = tid; q < t.groups; q += threads)
-            to_slots[q] = make_float4(pivot[q].x, sum[q].x, pivot[q].y, 0.0f);
+            slots[(uint64_t)(blockIdx.x + u) * p.gl + q] = make_float4(pivot[q].x, sum[q].x, pivot[q].y, 0.0f);
+        w = to;
     }
 
     cooperative_groups::this_grid().sync();
 
     const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
     const float m = (float)(a.pixels * a.per);
-    const uint32_t resident = all > p.ring ? all - p.ring : 0;  // rows of the run from here on are in the ring
-    if (resident) ahead.start(a, p, run.w0 + resident - 1);
-    Place<V> here;
-    if (all) here.start(a, p, run.w1 - 1);
-    slot = all ? (all - 1) % p.ring : 0;
-    to_slot = resident ? (resident - 1) % p.ring : 0;
+    const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
+    uint32_t next = all - 1;                                    // the batch that `ahead` is at
+    ahead.u = (run.w1 - 1) / p.rows;
+    ahead.unit(a, p, run, true);
+    while (next >= resident && next > 0) {
+        ahead.before(a, p, run);
+        --next;
+    }
+    slot = (all - 1) % p.ring;
+    to_slot = next % p.ring;
     for (uint32_t end = run.w1; end > run.w0;) {
         const uint32_t u = (end - 1) / p.rows, from = max(u * p.rows, run.w0);
         const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
         const Segment g = segment_of<V>(a, p, u, from, end, t);
         Lanes<T, V, L> lanes;
         if (g.cnt) lanes.load(a, g.c);
-        // Joined about a pivot, the mean of the unit's first segment: its share of the values bounds how far off it is.
-        uint32_t b0, b1;
-        runs_of_unit(p, u, b0, b1);
-        __syncthreads();  // sum and pivot are read no more
-        for (uint32_t q = tid; q < t.groups; q += threads) pivot[q].x = __ldcg(slots + (uint64_t)(b0 + u) * p.gl + q).x;
-        __syncthreads();
+        // Joined about a pivot, the mean of this block's own segment: its share of the values bounds how far off it is.
+        if (end != run.w1) {
+            __syncthreads();  // sum and pivot are read no more
+            for (uint32_t q = tid; q < t.groups; q += threads)
+                pivot[q].x = __ldcg(slots + (uint64_t)(blockIdx.x + u) * p.gl + q).x;
+            __syncthreads();
+        }
         join_runs<V>(a, p, t, g.n, part, sum, [&](uint64_t i, uint32_t q, float& s, float& s2) {
             const float4 v = __ldcg(slots + i);
             const float d = v.x - pivot[q].x;
@@ -269,29 +291,42 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
         }
         __syncthreads();
         if (g.cnt) lanes.fold(a, p, t, g.c, sum);
-#pragma unroll 2
-        for (uint32_t i = g.iters; i-- > 0;) {
-            --end;
+        uint64_t at = g.at + (g.iters - 1) / R * R * step;
+        const auto give = [&](const Pack<T, V>& v, uint64_t where) {
+            float f[V];
+            v.get(f);
+            lanes.template apply<ACT>(f);
+            if (DROP) drop_vector<V>(a.drop, dstep, where, f);
+            Pack<T, V> o;
+            o.set(f);
+            o.store((T*)a.out + where);
+        };
+        for (uint32_t i0 = (g.iters - 1) / R * R;; i0 -= R) {
+            --batch;
             copy_wait<F - 1>();
-            if (i < g.cnt) {
-                float f[V];
-                ring[slot * threads].get(f);
-                lanes.template apply<ACT>(f);
-                const uint64_t at = here.at(p);
-                if (DROP) drop_vector<V>(a.drop, dstep, at, f);
-                Pack<T, V> o;
-                o.set(f);
-                o.store((T*)a.out + at);
+            const Pack<T, V>* have = ring + slot * R * threads;
+            if (i0 + R <= g.cnt) {
+#pragma unroll
+                for (int j = 0; j < R; ++j) give(have[j * threads], at + j * step);
+            } else {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    if (i0 + j < g.cnt) give(have[j * threads], at + j * step);
             }
+            at -= R * step;
             slot = slot == 0 ? p.ring - 1 : slot - 1;
-            if (end != run.w0) here.before(a, p);
-            if (end - run.w0 >= F && end - run.w0 - F < resident) {  // the row F places before
+            if (batch == next + F && next < resident) {
                 copy();
-                if (end - run.w0 > F) ahead.before(a, p);
                 to_slot = to_slot == 0 ? p.ring - 1 : to_slot - 1;
+                if (next > 0) {
+                    ahead.before(a, p, run);
+                    --next;
+                }
             }
             copy_commit();
+            if (i0 == 0) break;
         }
+        end = from;
     }
 }
 

@@ -83,9 +83,12 @@ cudaError_t launch_one(const Call& c) {
         p.per_block = (total + blocks - 1) / blocks;
         blocks = (total + p.per_block - 1) / p.per_block;
     }
-    p.ring = (kSharedMost - 16 - head) / row;
-    if (p.ring > p.per_block) p.ring = p.per_block;
-    const uint32_t bytes = head + 16 + p.ring * row;
+    const uint32_t rows = c.bwd ? kRowsBwd : kRows, batch = rows * row;
+    // the longest run's batches: its rows, and a cut batch at each end of a unit
+    const uint32_t longest = p.per_block / rows + 1 + (p.per_unit ? 0 : p.per_block / p.rows + 1);
+    p.ring = (kSharedMost - 16 - head) / batch;
+    if (p.ring > longest) p.ring = longest;
+    const uint32_t bytes = head + 16 + p.ring * batch;
     if (c.bwd) {
         static std::atomic<uint64_t> done{0};
         auto k = large_bwd_kernel<T, V, L, ACT, DROP>;

@@ -120,7 +120,7 @@ class GroupNorm:
         g, _, w = _gate(z, self.act)
         y = z * g
         # the slope of z gate(z) stays below 1.13
-        t = 1.13 * t_z + y.abs() * (12 + 4 * w.abs()) * U + z.abs() * 2.0**-125  # gates below 2^-126 become 0
+        t = 1.13 * t_z + y.abs() * (12 + 4 * w.abs()) * U + z.abs() * 2.0**-60 * (w < -41)  # gates stop at 2^-60
         y, t = self._drop(y), t * self.scale * (1 + 2 * U)
         if self.keep is not None:
             t = torch.where(self.keep, t, torch.zeros_like(t))
@@ -136,7 +136,7 @@ class GroupNorm:
         slope = g + z * g * (1 - g) * dw
         # second derivative below 1.2; the slope's own roundings, with the exponential's
         t_slope = 1.2 * t_z + (16 + 8 * w.abs()) * U * (1 + (z * dw).abs() * (1 - g) * g * 4)
-        t_slope = t_slope + (1 + (z * dw).abs()) * 2.0**-125  # gates below 2^-126 become 0
+        t_slope = t_slope + (1 + (z * dw).abs()) * 2.0**-60 * (w < -41)  # gates stop at 2^-60
         dz = v * slope
         t_dz = v.abs() * t_slope + 4 * U * dz.abs()
         chain = (64 + self.x.shape[1] / 128) * U
