@@ -78,6 +78,8 @@ bool plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t
     }
     p.last = (uint32_t)(p.vecs - (uint64_t)(p.rows - 1) * p.rv);
     p.tiles = (p.rv + p.cols - 1) / p.cols;
+    p.pixels = p.tiles > 1 ? 1 : p.rv * v / c;
+    p.pixels_last = p.tiles > 1 ? 1 : p.last * v / c;
     p.threads = (p.k * p.cols + 31) / 32 * 32;
     p.blocks = p.small ? (uint32_t)(n * p.tiles) : 0;
     p.gl = groups_of_tile(c, per, p.cols * v, p.tiles);

@@ -19,7 +19,7 @@ constexpr int kThreads = 512;         // most threads of a block
 constexpr int kBatch = 8;             // vectors a thread holds, small samples
 constexpr int kRows = 4, kAhead = 2;  // large samples: rows of a batch, batches in flight ahead of the one at work
 constexpr int kBatchBwd = 4;          // the same for the backward, of x and of v each
-constexpr int kRowsBwd = 2, kAheadBwd = 2;
+constexpr int kRowsBwd = 2, kAheadBwd = 3;
 constexpr uint32_t kMaxBlocks = 512;  // most blocks of a kernel that leaves partial sums
 
 // Division of x by d for x d < 2^32: with f = (2^32 + e) / d, 0 < e <= d, the product's high word is
@@ -60,8 +60,9 @@ struct Plan {
     uint32_t tiles;
     uint32_t k;          // small samples: rows a block takes at a time
     uint32_t gl;         // most groups of a tile
-    uint32_t per_block;  // large samples: rows of a block
-    uint32_t per_unit;   // blocks of a (tile, sample); 0: the rows of all of them are dealt to the blocks in order
+    uint32_t per_unit;   // large samples: blocks of a (tile, sample), which take its rows in turn; or 0:
+    uint32_t per_block;  // consecutive rows of a block, over tiles, samples and rows
+    uint32_t pixels, pixels_last;  // of a row and of a sample's last row
     uint32_t ring;       // batches in shared memory
     uint32_t threads, blocks;
     uint32_t v;          // elements of a vector
@@ -297,13 +298,35 @@ __device__ __forceinline__ void group_span(const Args& a, const Tile& t, uint32_
     hi = (min(first + a.per, t.c1) - t.c0) / (V / L);
 }
 
+// A thread's part in the sums over the tile's groups: the items of group `q` that it walks.
+struct GroupWalk {
+    uint32_t q, l;        // group, and place among the group's t.lanes threads
+    uint32_t at, m, i;    // first item, its copy and place in the group
+    uint32_t dm, di, width;
+};
+template <int V, int L>
+__device__ __forceinline__ GroupWalk group_walk(const Args& a, const Tile& t, uint32_t u) {
+    GroupWalk w;
+    w.q = u >> t.log, w.l = u & (t.lanes - 1);
+    uint32_t lo, hi;
+    group_span<V, L>(a, t, min(w.q, t.groups - 1), lo, hi);
+    w.width = hi - lo;
+    const float inv = 1.0f / (float)w.width;  // quotients below 2^10, half a unit from the next: exact
+    w.m = (uint32_t)(((float)w.l + 0.5f) * inv);
+    w.i = w.l - w.m * w.width;
+    w.at = w.m * t.stride + lo + w.i;
+    w.dm = (uint32_t)(((float)t.lanes + 0.5f) * inv);
+    w.di = t.lanes - w.dm * w.width;
+    return w;
+}
+
 // Sums over the tile's groups of one value per item (thread t holds items t L ... t L + L - 1 of the block's
-// rows), in a fixed order: t.lanes threads walk each group's items. Afterwards sum[q] holds group g0 + q for all
-// threads. Starts without a barrier (whoever read part or sum last has passed one since, or passes the first one
-// here before they are written); ends with one.
+// rows), in a fixed order: t.lanes threads walk each group's items (`mine`: group_walk of the thread). Afterwards
+// sum[q] holds group g0 + q for all threads. Starts without a barrier (whoever read part or sum last has passed one
+// since, or passes the first one here before they are written); ends with one.
 template <int V, int L, bool PAIR>
-__device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const float (&x)[L], const float (&y)[L],
-                                           bool active, float* part, float2* warp_sum, float2* sum) {
+__device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const GroupWalk& mine, const float (&x)[L],
+                                           const float (&y)[L], bool active, float* part, float2* warp_sum, float2* sum) {
     const uint32_t tid = threadIdx.x, half = blockDim.x * L;  // half: the pair's second values
 #pragma unroll
     for (int j = 0; j < L; ++j) {
@@ -313,28 +336,23 @@ __device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const f
     __syncthreads();
     const uint32_t in = min(t.lanes, 32u);
     for (uint32_t base = 0; base < t.groups * t.lanes; base += blockDim.x) {
-        const uint32_t u = base + tid, q = u >> t.log, l = u & (t.lanes - 1);
+        GroupWalk w = mine;
+        if (base) w = group_walk<V, L>(a, t, base + tid);
         float s = 0.0f, s2 = 0.0f;
-        if (q < t.groups) {
-            uint32_t lo, hi;
-            group_span<V, L>(a, t, q, lo, hi);
-            const uint32_t width = hi - lo;
-            uint32_t m = (uint32_t)(((float)l + 0.5f) / (float)width), i = l - m * width;  // l < 2^9, exact
-            const uint32_t dm = (uint32_t)(((float)t.lanes + 0.5f) / (float)width), di = t.lanes - dm * width;
-            while (m < t.copies) {
-                const uint32_t at = m * t.stride + lo + i;
-                s += part[at];
-                if (PAIR) s2 += part[half + at];
-                m += dm, i += di;
-                if (i >= width) i -= width, ++m;
+        if (w.q < t.groups)
+            while (w.m < t.copies) {
+                s += part[w.at];
+                if (PAIR) s2 += part[half + w.at];
+                w.m += w.dm, w.i += w.di;
+                w.at += w.dm * t.stride + w.di;
+                if (w.i >= w.width) w.i -= w.width, ++w.m, w.at += t.stride - w.width;
             }
-        }
         for (uint32_t o = in / 2; o; o /= 2) {
             s += __shfl_xor_sync(~0u, s, o);
             if (PAIR) s2 += __shfl_xor_sync(~0u, s2, o);
         }
         if (t.lanes <= 32) {
-            if (l == 0 && q < t.groups) sum[q] = make_float2(s, s2);
+            if (w.l == 0 && w.q < t.groups) sum[w.q] = make_float2(s, s2);
         } else if ((tid & 31) == 0) {
             warp_sum[tid / 32] = make_float2(s, s2);
         }
@@ -363,19 +381,29 @@ __device__ __forceinline__ uint32_t channel_at(const Args& a, uint32_t c, int j)
 }
 
 // Large samples. Rows are whole block iterations, numbered over tiles, samples ("units") and rows. A block has
-// a run of them; a segment is its part of one unit.
+// parts of the units first ... last ("segments"): every per_unit-th row of one unit, or consecutive rows.
 struct Run {
-    uint32_t w0, w1;
+    uint32_t first, last;
+    uint32_t w0, w1;  // consecutive rows
+    uint32_t stride;  // rows from one to the next
 };
 __device__ __forceinline__ Run run_of(const Args& a, const Plan& p, uint32_t b) {
-    if (p.per_unit) {
-        const uint32_t u = b / p.per_unit, r = (b - u * p.per_unit) * p.per_block;
-        return {u * p.rows + min(r, p.rows), u * p.rows + min(r + p.per_block, p.rows)};
-    }
-    const uint32_t total = p.rows * (uint32_t)a.n * p.tiles;
-    return {b * p.per_block, min((b + 1) * p.per_block, total)};
+    if (p.per_unit) return {b / p.per_unit, b / p.per_unit, b % p.per_unit, 0, p.per_unit};
+    const uint32_t total = p.rows * (uint32_t)a.n * p.tiles, w0 = b * p.per_block, w1 = min(w0 + p.per_block, total);
+    return {w0 / p.rows, (w1 - 1) / p.rows, w0, w1, 1};
 }
-// Blocks whose runs meet unit u: [b0, b1].
+// Rows r0, r0 + stride, ... of unit u in a run.
+__device__ __forceinline__ void rows_of(const Plan& p, const Run& run, uint32_t u, uint32_t& r0, uint32_t& iters) {
+    if (p.per_unit) {
+        r0 = run.w0;
+        iters = (p.rows - r0 + run.stride - 1) / run.stride;
+    } else {
+        const uint32_t from = max(u * p.rows, run.w0);
+        r0 = from - u * p.rows;
+        iters = min((u + 1) * p.rows, run.w1) - from;
+    }
+}
+// Blocks that have rows of unit u: [b0, b1].
 __device__ __forceinline__ void runs_of_unit(const Plan& p, uint32_t u, uint32_t& b0, uint32_t& b1) {
     if (p.per_unit) {
         b0 = u * p.per_unit;
@@ -387,71 +415,67 @@ __device__ __forceinline__ void runs_of_unit(const Plan& p, uint32_t u, uint32_t
 }
 struct Segment {
     uint32_t n, tile, c;      // sample, tile, channel of the thread's first element
-    uint32_t r0, iters, cnt;  // rows [r0, r0 + iters); cnt: of this thread, which misses at most a sample's last row
+    uint32_t r0, iters, cnt;  // first row, rows, rows of this thread: it misses at most a sample's last row
     uint64_t at;              // first element of the thread's vector in row r0
     float pixels;
 };
 template <int V>
-__device__ __forceinline__ Segment segment_of(const Args& a, const Plan& p, uint32_t u, uint32_t from, uint32_t to,
-                                              const Tile& t) {
+__device__ __forceinline__ Segment segment_of(const Args& a, const Plan& p, const Run& run, uint32_t u, const Tile& t) {
     Segment s;
     s.tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n;
     s.n = u - s.tile * (uint32_t)a.n;
-    s.r0 = from - u * p.rows;
-    s.iters = to - from;
+    rows_of(p, run, u, s.r0, s.iters);
     const uint32_t col = s.tile * p.cols + threadIdx.x;
-    const bool ends = s.r0 + s.iters == p.rows;
+    const bool ends = s.r0 + (s.iters - 1) * run.stride + 1 == p.rows;
     s.cnt = threadIdx.x < t.cols ? s.iters - (ends && col >= p.last) : 0;
     s.at = (s.n * p.vecs + (uint64_t)s.r0 * p.rv + col) * V;
     s.c = col * V;
     if (p.tiles == 1) s.c -= p.by_c(s.c) * a.c;
-    s.pixels = p.tiles > 1 ? (float)s.iters
-                           : (float)(uint64_t)(((uint64_t)(s.iters - ends) * p.rv + (ends ? p.last : 0)) * V / a.c);
+    s.pixels = (float)(s.iters - ends) * (float)p.pixels + (ends ? (float)p.pixels_last : 0.0f);
     return s;
 }
-// Batches of R rows of a run, each inside one segment, counted from the segment's first row.
+// Batches of R rows of a run, each inside one segment.
 template <int R>
 __device__ __forceinline__ uint32_t batches_of(const Plan& p, const Run& run) {
     uint32_t all = 0;
-    for (uint32_t w = run.w0; w < run.w1;) {
-        const uint32_t to = min((w / p.rows + 1) * p.rows, run.w1);
-        all += (to - w + R - 1) / R;
-        w = to;
+    for (uint32_t u = run.first; u <= run.last; ++u) {
+        uint32_t r0, iters;
+        rows_of(p, run, u, r0, iters);
+        all += (iters + R - 1) / R;
     }
     return all;
 }
 // The batch that is copied next: a walk over a run's batches, forwards or backwards.
 template <int V, int R>
 struct Walk {
-    uint32_t u, w, from, to, valid;  // unit; first row; the segment; end of the rows in which the thread has a vector
-    uint64_t at;                     // element of row w
+    uint32_t u, i, iters, valid;  // unit; first row of the batch, of the segment's iters; rows in which the thread has a vector
+    uint64_t at;                  // element of row i
 
     __device__ __forceinline__ void unit(const Args& a, const Plan& p, const Run& run, bool last) {
-        from = max(u * p.rows, run.w0);
-        to = min((u + 1) * p.rows, run.w1);
-        w = last ? from + (to - 1 - from) / R * R : from;
+        uint32_t r0;
+        rows_of(p, run, u, r0, iters);
+        i = last ? (iters - 1) / R * R : 0;
         const uint32_t tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n, n = u - tile * (uint32_t)a.n;
         const uint32_t col = tile * p.cols + threadIdx.x;
-        valid = threadIdx.x < p.cols && col < p.rv ? to - (to == (u + 1) * p.rows && col >= p.last) : 0;
-        at = (n * p.vecs + (uint64_t)(w - u * p.rows) * p.rv + col) * V;
+        const bool ends = r0 + (iters - 1) * run.stride + 1 == p.rows;
+        valid = threadIdx.x < p.cols && col < p.rv ? iters - (ends && col >= p.last) : 0;
+        at = (n * p.vecs + (uint64_t)(r0 + i * run.stride) * p.rv + col) * V;
     }
-    __device__ __forceinline__ void next(const Args& a, const Plan& p, const Run& run) {
-        w += R;
-        at += (uint64_t)(R * V) * p.rv;
-        if (w >= to && to < run.w1) {
+    __device__ __forceinline__ void next(const Args& a, const Plan& p, const Run& run, uint64_t step) {
+        i += R;
+        at += R * step;
+        if (i >= iters && u < run.last) {
             ++u;
             unit(a, p, run, false);
         }
     }
-    __device__ __forceinline__ void before(const Args& a, const Plan& p, const Run& run) {
-        if (w == from) {
-            if (from > run.w0) {
-                --u;
-                unit(a, p, run, true);
-            }
-        } else {
-            w -= R;
-            at -= (uint64_t)(R * V) * p.rv;
+    __device__ __forceinline__ void before(const Args& a, const Plan& p, const Run& run, uint64_t step) {
+        if (i) {
+            i -= R;
+            at -= R * step;
+        } else if (u > run.first) {
+            --u;
+            unit(a, p, run, true);
         }
     }
 };

@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
     const float m = (float)(a.pixels * a.per);
     GradLanes<T, V, L> lanes;
     if (active) lanes.load(a, c);
+    const GroupWalk walk = group_walk<V, L>(a, t, tid);
     float acc_a[V] = {}, acc_b[V] = {};
     for (uint32_t n = blockIdx.x / p.tiles; n < a.n; n += gridDim.x / p.tiles) {
         const uint64_t at = (n * p.vecs + row * p.rv + col) * V;
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
         float i1[L], i2[L];
         per_item<V, L>(s1, i1);
         per_item<V, L>(s2, i2);
-        group_sums<V, L, true>(a, t, i1, i2, active, part, warp_sum, sum);
+        group_sums<V, L, true>(a, t, walk, i1, i2, active, part, warp_sum, sum);
         if (cnt) {
             GroupGrad<T, V, L> gg;
             gg.take(a, p, t, c, sum, m, lanes);
@@ -220,8 +221,8 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
     float2* chan = sum + p.gl;              // [tile_c]
     float* part = (float*)(chan + tile_c);  // [2][threads][V]
     Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + threads * 2 * V) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][x, v][threads]
-    const uint64_t step = (uint64_t)p.rv * V;
     const Run run = run_of(a, p, blockIdx.x);
+    const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
     const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
     float2* slots = (float2*)a.ws;                                                   // [(block + unit) gl + group]
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
     const bool wanted = a.v_weight || a.v_bias;
 
     Walk<V, R> ahead;
-    ahead.u = run.w0 / p.rows;
+    ahead.u = run.first;
     ahead.unit(a, p, run, false);
     uint32_t to_slot = 0, slot = 0;
     const auto copy = [&]() {
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
         const T *x = (const T*)a.x + ahead.at, *v = (const T*)a.v + ahead.at;
 #pragma unroll
         for (int j = 0; j < R; ++j)
-            if (ahead.w + j < ahead.valid) {
+            if (ahead.i + j < ahead.valid) {
                 copy_async<T, V>(to + 2 * j * threads, x + j * step);
                 copy_async<T, V>(to + (2 * j + 1) * threads, v + j * step);
             }
@@ -246,18 +247,19 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
     for (uint32_t b = 0; b < F; ++b) {
         if (b < all) {
             copy();
-            ahead.next(a, p, run);
+            ahead.next(a, p, run, step);
             to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
         }
         copy_commit();
     }
     uint32_t batch = 0;
     bool first = true;  // first segment of the block in its tile
-    for (uint32_t w = run.w0; w < run.w1;) {
-        const uint32_t u = w / p.rows, to = min((u + 1) * p.rows, run.w1);
-        const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
-        const Segment g = segment_of<V>(a, p, u, w, to, t);
-        GradLanes<T, V, L> lanes;
+    Tile t;
+    Segment g;
+    GradLanes<T, V, L> lanes;
+    for (uint32_t u = run.first; u <= run.last; ++u) {
+        t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
+        g = segment_of<V>(a, p, run, u, t);
         if (g.cnt) {
             lanes.load(a, g.c);
             lanes.stats(a, p, g.n, g.c);
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             slot = slot + 1 == p.ring ? 0 : slot + 1;
             if (batch + F < all) {
                 copy();
-                ahead.next(a, p, run);
+                ahead.next(a, p, run, step);
                 to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
             }
             copy_commit();
@@ -331,34 +333,35 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             to_slots[q] = make_float2(s1, s2);
         }
         __syncthreads();
-        w = to;
-        first = p.tiles > 1 && w / p.rows / (uint32_t)a.n != g.tile;
+        first = p.tiles > 1 && (u + 1) / (uint32_t)a.n != g.tile;
     }
 
-    cooperative_groups::this_grid().sync();
-
+    // What the second pass needs and no other block gives.
     const float m = (float)(a.pixels * a.per);
     const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
     uint32_t next = all - 1;                                    // the batch that `ahead` is at
-    ahead.u = (run.w1 - 1) / p.rows;
+    ahead.u = run.last;
     ahead.unit(a, p, run, true);
     while (next >= resident && next > 0) {
-        ahead.before(a, p, run);
+        ahead.before(a, p, run, step);
         --next;
     }
     slot = (all - 1) % p.ring;
     to_slot = next % p.ring;
-    for (uint32_t end = run.w1; end > run.w0;) {
-        const uint32_t u = (end - 1) / p.rows, from = max(u * p.rows, run.w0);
-        const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
-        const Segment g = segment_of<V>(a, p, u, from, end, t);
-        GradLanes<T, V, L> lanes;
-        GroupGrad<T, V, L> gg;
-        if (g.cnt) {
-            lanes.load(a, g.c);
-            lanes.stats(a, p, g.n, g.c);
+
+    cooperative_groups::this_grid().sync();
+
+    for (uint32_t u = run.last;; --u) {
+        if (u != run.last) {
+            t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
+            g = segment_of<V>(a, p, run, u, t);
+            if (g.cnt) {
+                lanes.load(a, g.c);
+                lanes.stats(a, p, g.n, g.c);
+            }
+            __syncthreads();  // sum of the segment before is read no more
         }
-        __syncthreads();  // sum of the segment before is read no more
+        GroupGrad<T, V, L> gg;
         join_runs<V>(a, p, t, g.n, part, sum, [&](uint64_t i, uint32_t, float& s1, float& s2) {
             const float2 v = __ldcg(slots + i);
             s1 += v.x;
@@ -395,14 +398,14 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
                 copy();
                 to_slot = to_slot == 0 ? p.ring - 1 : to_slot - 1;
                 if (next > 0) {
-                    ahead.before(a, p, run);
+                    ahead.before(a, p, run, step);
                     --next;
                 }
             }
             copy_commit();
             if (i0 == 0) break;
         }
-        end = from;
+        if (u == run.first) break;
     }
     if (wanted)
         for (uint32_t ch = blockIdx.x * (threads / 32) + tid / 32; ch < a.c; ch += gridDim.x * (threads / 32)) {

@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
     const uint32_t c = p.tiles > 1 ? col * V : col * V - p.by_c(col * V) * a.c;
     Lanes<T, V, L> lanes;
     if (active) lanes.load(a, c);
+    const GroupWalk walk = group_walk<V, L>(a, t, tid);
 
     constexpr int P = kParts<V, L>;
     const float m = (float)(a.pixels * a.per);  // values of a group
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
             accumulate<V, P>(acc, f);
         }
     per_item<V, L>(acc, val);
-    group_sums<V, L, false>(a, t, val, val, active, part, warp_sum, sum);
+    group_sums<V, L, false>(a, t, walk, val, val, active, part, warp_sum, sum);
 #pragma unroll
     for (int j = 0; j < L; ++j) off[j] = active ? -sum[p.by_per(channel_at<L>(a, c, j)) - t.g0].x / m : 0.0f;
     for (uint32_t q = tid; q < t.groups; q += blockDim.x) means[q] = sum[q].x / m;
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
             accumulate<V, P>(acc, f, f);
         }
     per_item<V, L>(acc, val);
-    group_sums<V, L, false>(a, t, val, val, active, part, warp_sum, sum);
+    group_sums<V, L, false>(a, t, walk, val, val, active, part, warp_sum, sum);
     for (uint32_t q = tid; q < t.groups; q += blockDim.x) {
         const float rstd = 1.0f / sqrtf(sum[q].x / m + a.eps);
         sum[q] = make_float2(means[q], rstd);
@@ -132,41 +133,43 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
     const uint32_t tid = threadIdx.x, threads = blockDim.x;
     Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + threads * (L > 2 ? L : 2)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][threads]
     constexpr int P = kParts<V, L>, R = kRows, F = kAhead;
-    const uint64_t step = (uint64_t)p.rv * V;
     const Run run = run_of(a, p, blockIdx.x);
+    const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
     float4* slots = (float4*)a.ws;  // [(block + unit) gl + group]: mean, squared deviations, count
 
     Walk<V, R> ahead;
-    ahead.u = run.w0 / p.rows;
+    ahead.u = run.first;
     ahead.unit(a, p, run, false);
     uint32_t to_slot = 0, slot = 0;  // ring places of the batch to copy and of the batch at work
     const auto copy = [&]() {
         Pack<T, V>* to = ring + to_slot * R * threads;
         const T* x = (const T*)a.x + ahead.at;
-        if (ahead.w + R <= ahead.valid) {
+        if (ahead.i + R <= ahead.valid) {
 #pragma unroll
             for (int j = 0; j < R; ++j) copy_async<T, V>(to + j * threads, x + j * step);
         } else {
 #pragma unroll
             for (int j = 0; j < R; ++j)
-                if (ahead.w + j < ahead.valid) copy_async<T, V>(to + j * threads, x + j * step);
+                if (ahead.i + j < ahead.valid) copy_async<T, V>(to + j * threads, x + j * step);
         }
     };
 #pragma unroll 1
     for (uint32_t b = 0; b < F; ++b) {
         if (b < all) {
             copy();
-            ahead.next(a, p, run);
+            ahead.next(a, p, run, step);
             to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
         }
         copy_commit();
     }
     uint32_t batch = 0;
-    for (uint32_t w = run.w0; w < run.w1;) {
-        const uint32_t u = w / p.rows, to = min((u + 1) * p.rows, run.w1);
-        const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
-        const Segment g = segment_of<V>(a, p, u, w, to, t);
+    Tile t;
+    Segment g;
+    for (uint32_t u = run.first; u <= run.last; ++u) {
+        t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
+        g = segment_of<V>(a, p, run, u, t);
+        const GroupWalk walk = group_walk<V, L>(a, t, tid);
         float off[L] = {}, acc[P] = {}, sq[P] = {};
         const auto take = [&](const Pack<T, V>& v) {
             float f[V];
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
             slot = slot + 1 == p.ring ? 0 : slot + 1;
             if (batch + F < all) {
                 copy();
-                ahead.next(a, p, run);
+                ahead.next(a, p, run, step);
                 to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
             }
             copy_commit();
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
             if (dev[j] < 0.0f) dev[j] = 0.0f;  // rounding; NaN stays
             val[j] = cnt * mean[j];
         }
-        group_sums<V, L, false>(a, t, val, val, g.cnt != 0, part, warp_sum, sum);
+        group_sums<V, L, false>(a, t, walk, val, val, g.cnt != 0, part, warp_sum, sum);
         for (uint32_t q = tid; q < t.groups; q += threads) {
             uint32_t lo, hi;
             group_span<V, V>(a, t, q, lo, hi);
@@ -238,39 +241,40 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
                 val[j] = __fmaf_rn(cnt * d, d, dev[j]);
             }
         }
-        group_sums<V, L, false>(a, t, val, val, g.cnt != 0, part, warp_sum, sum);
+        group_sums<V, L, false>(a, t, walk, val, val, g.cnt != 0, part, warp_sum, sum);
         for (uint32_t q = tid; q < t.groups; q += threads)
             slots[(uint64_t)(blockIdx.x + u) * p.gl + q] = make_float4(pivot[q].x, sum[q].x, pivot[q].y, 0.0f);
-        w = to;
     }
 
-    cooperative_groups::this_grid().sync();
-
+    // What the second pass needs and no other block gives.
     const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
     const float m = (float)(a.pixels * a.per);
     const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
     uint32_t next = all - 1;                                    // the batch that `ahead` is at
-    ahead.u = (run.w1 - 1) / p.rows;
+    ahead.u = run.last;
     ahead.unit(a, p, run, true);
     while (next >= resident && next > 0) {
-        ahead.before(a, p, run);
+        ahead.before(a, p, run, step);
         --next;
     }
     slot = (all - 1) % p.ring;
     to_slot = next % p.ring;
-    for (uint32_t end = run.w1; end > run.w0;) {
-        const uint32_t u = (end - 1) / p.rows, from = max(u * p.rows, run.w0);
-        const Tile t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
-        const Segment g = segment_of<V>(a, p, u, from, end, t);
-        Lanes<T, V, L> lanes;
-        if (g.cnt) lanes.load(a, g.c);
-        // Joined about a pivot, the mean of this block's own segment: its share of the values bounds how far off it is.
-        if (end != run.w1) {
+    Lanes<T, V, L> lanes;
+    if (g.cnt) lanes.load(a, g.c);
+
+    cooperative_groups::this_grid().sync();
+
+    for (uint32_t u = run.last;; --u) {
+        if (u != run.last) {
+            t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
+            g = segment_of<V>(a, p, run, u, t);
+            if (g.cnt) lanes.load(a, g.c);
             __syncthreads();  // sum and pivot are read no more
             for (uint32_t q = tid; q < t.groups; q += threads)
                 pivot[q].x = __ldcg(slots + (uint64_t)(blockIdx.x + u) * p.gl + q).x;
             __syncthreads();
         }
+        // Joined about a pivot, the mean of this block's own segment: its share of the values bounds how far off it is.
         join_runs<V>(a, p, t, g.n, part, sum, [&](uint64_t i, uint32_t q, float& s, float& s2) {
             const float4 v = __ldcg(slots + i);
             const float d = v.x - pivot[q].x;
@@ -319,14 +323,14 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
                 copy();
                 to_slot = to_slot == 0 ? p.ring - 1 : to_slot - 1;
                 if (next > 0) {
-                    ahead.before(a, p, run);
+                    ahead.before(a, p, run, step);
                     --next;
                 }
             }
             copy_commit();
             if (i0 == 0) break;
         }
-        end = from;
+        if (u == run.first) break;
     }
 }
 

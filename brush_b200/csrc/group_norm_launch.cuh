@@ -69,14 +69,13 @@ cudaError_t launch_one(const Call& c) {
     const uint32_t tile_c = p.tiles == 1 ? a.c : p.cols * V;
     const uint32_t head = c.bwd ? 8 * (p.gl + tile_c + p.threads * V) : sums + 8 * p.gl + 4 * p.threads * (L > 2 ? L : 2);
     const uint32_t row = p.threads * (uint32_t)sizeof(Pack<T, V>) * (c.bwd ? 2 : 1);  // a single 16-bit element takes a word
-    // Runs: where units are few, each has blocks of its own, so that no block sums and joins twice; where that
-    // would leave more than a tenth of the SMs idle, runs cross units.
+    // Where units are few, each has blocks of its own, so that no block sums and joins twice; where that would
+    // leave more than a tenth of the SMs idle, runs cross units.
     const uint32_t units = (uint32_t)a.n * p.tiles, total = p.rows * units;
     uint32_t blocks = total < (uint32_t)sms ? total : (uint32_t)sms;
     p.per_unit = blocks / units;
     if (p.per_unit > 0 && p.per_unit * units * 10 >= blocks * 9) {
         p.per_block = (p.rows + p.per_unit - 1) / p.per_unit;
-        p.per_unit = (p.rows + p.per_block - 1) / p.per_block;
         blocks = p.per_unit * units;
     } else {
         p.per_unit = 0;
