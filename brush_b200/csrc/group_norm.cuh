@@ -298,6 +298,25 @@ __device__ __forceinline__ void group_span(const Args& a, const Tile& t, uint32_
     hi = (min(first + a.per, t.c1) - t.c0) / (V / L);
 }
 
+// Place of an item in shared memory: with several items a thread, four words more every 32, so that threads write
+// 16 bytes at a time and the walks over copies of a channel meet other banks.
+template <int L>
+__device__ __forceinline__ uint32_t place(uint32_t e) { return L > 1 ? e + (e >> 5) * 4 : e; }
+template <int L>
+__host__ __device__ constexpr uint32_t places(uint32_t threads) { return L > 1 ? threads * L + threads * L / 8 : threads; }
+template <int L>
+__device__ __forceinline__ void put_items(float* part, const float (&x)[L], bool active) {
+    if constexpr (L >= 4) {
+        float4* to = (float4*)(part + place<L>(threadIdx.x * L));  // L items lie in one run of 32
+#pragma unroll
+        for (int j = 0; j < L; j += 4)
+            to[j / 4] = active ? make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < L; ++j) part[place<L>(threadIdx.x * L + j)] = active ? x[j] : 0.0f;
+    }
+}
+
 // A thread's part in the sums over the tile's groups: the items of group `q` that it walks.
 struct GroupWalk {
     uint32_t q, l;        // group, and place among the group's t.lanes threads
@@ -327,12 +346,9 @@ __device__ __forceinline__ GroupWalk group_walk(const Args& a, const Tile& t, ui
 template <int V, int L, bool PAIR>
 __device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const GroupWalk& mine, const float (&x)[L],
                                            const float (&y)[L], bool active, float* part, float2* warp_sum, float2* sum) {
-    const uint32_t tid = threadIdx.x, half = blockDim.x * L;  // half: the pair's second values
-#pragma unroll
-    for (int j = 0; j < L; ++j) {
-        part[tid * L + j] = active ? x[j] : 0.0f;
-        if (PAIR) part[half + tid * L + j] = active ? y[j] : 0.0f;
-    }
+    const uint32_t tid = threadIdx.x, half = places<L>(blockDim.x);  // half: the pair's second values
+    put_items<L>(part, x, active);
+    if (PAIR) put_items<L>(part + half, y, active);
     __syncthreads();
     const uint32_t in = min(t.lanes, 32u);
     for (uint32_t base = 0; base < t.groups * t.lanes; base += blockDim.x) {
@@ -341,8 +357,8 @@ __device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const G
         float s = 0.0f, s2 = 0.0f;
         if (w.q < t.groups)
             while (w.m < t.copies) {
-                s += part[w.at];
-                if (PAIR) s2 += part[half + w.at];
+                s += part[place<L>(w.at)];
+                if (PAIR) s2 += part[half + place<L>(w.at)];
                 w.m += w.dm, w.i += w.di;
                 w.at += w.dm * t.stride + w.di;
                 if (w.i >= w.width) w.i -= w.width, ++w.m, w.at += t.stride - w.width;

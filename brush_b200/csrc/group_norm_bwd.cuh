@@ -62,13 +62,10 @@ struct GroupGrad {
 template <int V>
 __device__ __forceinline__ void channel_sums(const Tile& t, uint32_t items, const float (&x)[V], const float (&y)[V],
                                              bool active, float* part, float2* to) {
-    const uint32_t tid = threadIdx.x, half = blockDim.x * V;
+    const uint32_t tid = threadIdx.x, half = places<V>(blockDim.x);
     const uint32_t width = t.c1 - t.c0, copies = items * V / width;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        part[tid * V + j] = active ? x[j] : 0.0f;
-        part[half + tid * V + j] = active ? y[j] : 0.0f;
-    }
+    put_items<V>(part, x, active);
+    put_items<V>(part + half, y, active);
     __syncthreads();
     // q threads a channel sum every q-th copy into the first q copies, then one adds those
     uint32_t q = min(blockDim.x / width, copies);
@@ -77,11 +74,13 @@ __device__ __forceinline__ void channel_sums(const Tile& t, uint32_t items, cons
         if (z < q) {
             float s = 0.0f, s2 = 0.0f;
             for (uint32_t m = z; m < copies; m += q) {
-                s += part[m * width + i];
-                s2 += part[half + m * width + i];
+                const uint32_t at = place<V>(m * width + i);
+                s += part[at];
+                s2 += part[half + at];
             }
-            part[z * width + i] = s;
-            part[half + z * width + i] = s2;
+            const uint32_t at = place<V>(z * width + i);
+            part[at] = s;
+            part[half + at] = s2;
         }
         __syncthreads();
     } else {
@@ -90,8 +89,9 @@ __device__ __forceinline__ void channel_sums(const Tile& t, uint32_t items, cons
     for (uint32_t i = tid; i < width; i += blockDim.x) {
         float s = 0.0f, s2 = 0.0f;
         for (uint32_t m = 0; m < q; ++m) {
-            s += part[m * width + i];
-            s2 += part[half + m * width + i];
+            const uint32_t at = place<V>(m * width + i);
+            s += part[at];
+            s2 += part[half + at];
         }
         to[i] = make_float2(s, s2);
     }
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;                       // [gl]
     float2* warp_sum = sum + p.gl;                     // [warps]
-    float* part = (float*)(warp_sum + kThreads / 32);  // [2][threads][V]
+    float* part = (float*)(((uintptr_t)(warp_sum + kThreads / 32) + 15) & ~(uintptr_t)15);  // [2] places<V>
     constexpr int P = kParts<V, L>;
     const uint32_t tid = threadIdx.x, tile = blockIdx.x % p.tiles;
     const Tile t = tile_of<V, L>(a, p, tile);
@@ -219,8 +219,8 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
     const uint32_t tid = threadIdx.x, threads = blockDim.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;
     float2* sum = (float2*)smem;            // [gl]
     float2* chan = sum + p.gl;              // [tile_c]
-    float* part = (float*)(chan + tile_c);  // [2][threads][V]
-    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + threads * 2 * V) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][x, v][threads]
+    float* part = (float*)(((uintptr_t)(chan + tile_c) + 15) & ~(uintptr_t)15);  // [2] places<V>
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + 2 * places<V>(threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][x, v][threads]
     const Run run = run_of(a, p, blockIdx.x);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);

@@ -44,8 +44,8 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;           // [gl]
     float2* warp_sum = sum + p.gl;         // [warps]
-    float* means = (float*)(warp_sum + kThreads / 32);  // [gl]
-    float* part = means + p.gl;            // [threads][L]
+    float* part = (float*)(((uintptr_t)(warp_sum + kThreads / 32) + 15) & ~(uintptr_t)15);  // places<L>
+    float* means = part + places<L>(blockDim.x);  // [gl]
     const uint32_t tid = threadIdx.x;
     const uint32_t n = p.tiles == 1 ? blockIdx.x : blockIdx.x / p.tiles, tile = blockIdx.x - n * p.tiles;
     const Tile t = tile_of<V, L>(a, p, tile);
@@ -129,9 +129,9 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
     float2* sum = (float2*)smem;                       // [gl]
     float2* warp_sum = sum + p.gl;                     // [warps]
     float2* pivot = warp_sum + kThreads / 32;          // [gl]: mean and count of the block's last segment
-    float* part = (float*)(pivot + p.gl);              // [threads][max(L, 2)]
+    float* part = (float*)(((uintptr_t)(pivot + p.gl) + 15) & ~(uintptr_t)15);  // places<L>, two words a thread at least
     const uint32_t tid = threadIdx.x, threads = blockDim.x;
-    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + threads * (L > 2 ? L : 2)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][threads]
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + max(places<L>(threads), 2 * threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][threads]
     constexpr int P = kParts<V, L>, R = kRows, F = kAhead;
     const Run run = run_of(a, p, blockIdx.x);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;

@@ -52,14 +52,14 @@ cudaError_t launch_one(const Call& c) {
         static std::atomic<uint64_t> done{0};
         auto k = small_fwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
-        k<<<p.blocks, p.threads, sums + 4 * (p.gl + p.threads * L), c.stream>>>(a, p);
+        k<<<p.blocks, p.threads, sums + 16 + 4 * (p.gl + places<L>(p.threads)), c.stream>>>(a, p);
         return cudaSuccess;
     }
     if (p.small) {
         static std::atomic<uint64_t> done{0};
         auto k = small_bwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
-        const uint32_t bytes = sums + 8 * p.threads * V;
+        const uint32_t bytes = sums + 16 + 8 * places<V>(p.threads);
         int per_sm = 1;
         if (p.blocks > (uint32_t)sms)
             if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, (int)p.threads, bytes)) return e;
@@ -67,7 +67,8 @@ cudaError_t launch_one(const Call& c) {
         return cooperative(k, a, p, p.blocks < most ? p.blocks : most / p.tiles * p.tiles, bytes, c.stream);
     }
     const uint32_t tile_c = p.tiles == 1 ? a.c : p.cols * V;
-    const uint32_t head = c.bwd ? 8 * (p.gl + tile_c + p.threads * V) : sums + 8 * p.gl + 4 * p.threads * (L > 2 ? L : 2);
+    const uint32_t words = places<L>(p.threads) > 2 * p.threads ? places<L>(p.threads) : 2 * p.threads;
+    const uint32_t head = 16 + (c.bwd ? 8 * (p.gl + tile_c + places<V>(p.threads)) : sums + 8 * p.gl + 4 * words);
     const uint32_t row = p.threads * (uint32_t)sizeof(Pack<T, V>) * (c.bwd ? 2 : 1);  // a single 16-bit element takes a word
     // Where units are few, each has blocks of its own, so that no block sums and joins twice; where that would
     // leave more than a tenth of the SMs idle, runs cross units.
