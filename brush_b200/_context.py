@@ -77,11 +77,16 @@ def context(device: torch.device | int | None = None) -> Context:
     return ctx
 
 
-def feature_context(device: torch.device) -> tuple[Context, int]:
-    """(context, current stream) for the operators that take their stream as an argument; the
-    stream the context is bound to stays as it is."""
-    ctx = _CTX.get(device.index)
-    return ctx if ctx is not None else context(device), torch.cuda.current_stream(device).cuda_stream
+# The raw handle of a device's current stream; the public call builds a Stream object around it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def feature_context(index: int) -> tuple[Context, int]:
+    """(context, current stream) of a device for the operators that take their stream as an argument;
+    the stream the context is bound to stays as it is."""
+    ctx = _CTX.get(index)
+    return ctx if ctx is not None else context(index), _raw_stream(index)
 
 
 class _DeviceArray:

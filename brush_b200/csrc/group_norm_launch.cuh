@@ -60,9 +60,18 @@ cudaError_t launch_one(const Call& c) {
         auto k = small_bwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
         const uint32_t bytes = sums + 16 + 8 * places<V>(p.threads);
+        // blocks that fit an SM with these threads and bytes; the last answer is kept, a query costs as much as a launch
+        static std::atomic<uint64_t> known{0};
         int per_sm = 1;
-        if (p.blocks > (uint32_t)sms)
-            if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, (int)p.threads, bytes)) return e;
+        if (p.blocks > (uint32_t)sms) {
+            const uint64_t key = (uint64_t)p.threads << 40 | (uint64_t)bytes << 16, got = known.load();
+            if (got >> 16 << 16 == key) {
+                per_sm = (int)(got & 0xffff);
+            } else {
+                if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, (int)p.threads, bytes)) return e;
+                known.store(key | (uint64_t)per_sm);
+            }
+        }
         const uint32_t most = (uint32_t)(sms * per_sm) < kMaxBlocks ? (uint32_t)(sms * per_sm) : kMaxBlocks;
         return cooperative(k, a, p, p.blocks < most ? p.blocks : most / p.tiles * p.tiles, bytes, c.stream);
     }

@@ -9,7 +9,6 @@ rows of a ``[N, C]`` tensor (splats, or the rows of a residual branch).
 from __future__ import annotations
 
 import ctypes as C
-import math
 from dataclasses import dataclass
 
 import torch
@@ -31,21 +30,20 @@ class DropoutConfig:
     share: int = 1
 
     def to_c(self, device: torch.device) -> _lib.DropoutCfg:
-        p = float(self.p)
+        p, seed, step, share = self.p, self.seed, self.step, self.share
         if not 0.0 <= p <= 1.0:
-            raise ValueError(f"dropout p must lie in [0, 1], got {self.p}")
-        if not 0 <= self.seed < 1 << 64:
+            raise ValueError(f"dropout p must lie in [0, 1], got {p}")
+        if not 0 <= seed < 1 << 64:
             raise ValueError("dropout seed must be an unsigned 64-bit number")
-        if self.share < 1:
+        if share < 1:
             raise ValueError("dropout share must be at least 1")
-        step, d_step = self.step, None
         if isinstance(step, torch.Tensor):
             if step.dtype not in (torch.int32, torch.uint32) or step.numel() != 1 or step.device != device:
                 raise ValueError("a dropout step tensor must be one int32 element on the tensor's device")
-            step, d_step = 0, step.data_ptr()
-        elif not 0 <= step < 1 << 32:
+            return _lib.DropoutCfg(p, seed, share, step.data_ptr(), 0)
+        if not 0 <= step < 1 << 32:
             raise ValueError("dropout step must be an unsigned 32-bit number")
-        return _lib.DropoutCfg(p, self.seed, self.share, d_step, step)
+        return _lib.DropoutCfg(p, seed, share, None, step)
 
 
 def feature_tensor(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -54,34 +52,39 @@ def feature_tensor(t: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name} must be a float32, bfloat16 or float16 tensor")
     if not t.is_cuda:
         raise ValueError("bsx entry points take CUDA tensors")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def like_tensor(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
     """``t`` checked to have the shape, type and device of ``x``, contiguous."""
     if not isinstance(t, torch.Tensor) or t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
         raise ValueError(f"{name} must have the shape, type and device of the tensor it belongs to")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def dropout_forward(x: torch.Tensor, cfg: DropoutConfig, residual: torch.Tensor | None = None) -> torch.Tensor:
     """``residual + dropout(x)`` in x's shape and type; formed in 32 bits, rounded once."""
     x = feature_tensor(x, "x")
-    res = None if residual is None else like_tensor(residual, x, "residual")
-    ctx, stream = feature_context(x.device)
+    if residual is not None:
+        residual = like_tensor(residual, x, "residual")
     c = cfg.to_c(x.device)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ctx.check(_lib.lib().bsx_dropout_fwd(ctx.handle, x.data_ptr(), None if res is None else res.data_ptr(), x.numel(),
-                                         DTYPES[x.dtype], C.byref(c), out.data_ptr(), stream))
+    ctx, stream = feature_context(x.get_device())
+    out = torch.empty_like(x)
+    status = _lib.lib().bsx_dropout_fwd(ctx.handle, x.data_ptr(), None if residual is None else residual.data_ptr(),
+                                        x.numel(), DTYPES[x.dtype], C.byref(c), out.data_ptr(), stream)
+    if status:
+        ctx.check(status)
     return out
 
 
 def dropout_backward(v_output: torch.Tensor, cfg: DropoutConfig) -> torch.Tensor:
     """The gradient of x for ``v_output``; the residual's gradient is ``v_output`` itself."""
     v = feature_tensor(v_output, "v_output")
-    ctx, stream = feature_context(v.device)
     c = cfg.to_c(v.device)
-    v_x = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    ctx.check(_lib.lib().bsx_dropout_bwd(ctx.handle, v.data_ptr(), v.numel(), DTYPES[v.dtype], C.byref(c),
-                                         v_x.data_ptr(), stream))
+    ctx, stream = feature_context(v.get_device())
+    v_x = torch.empty_like(v)
+    status = _lib.lib().bsx_dropout_bwd(ctx.handle, v.data_ptr(), v.numel(), DTYPES[v.dtype], C.byref(c), v_x.data_ptr(),
+                                        stream)
+    if status:
+        ctx.check(status)
     return v_x

@@ -6,6 +6,7 @@ Statistics, gates and sums are formed in 32 bits whatever the tensor's type, and
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from dataclasses import dataclass
 
@@ -26,62 +27,80 @@ class GroupNormConfig:
     dropout: DropoutConfig | None = None    # after the activation, share 1
 
 
-def _call(x: torch.Tensor, weight, bias, cfg: GroupNormConfig):
-    """Checks what both directions share: (sizes, C configuration, what the call must keep alive)."""
-    if x.dim() < 2:
-        raise ValueError(f"x must be [N, ..., C], got {tuple(x.shape)}")
-    n, c = x.shape[0], x.shape[-1]
-    if cfg.groups < 1 or c < 1 or c % cfg.groups:
-        raise ValueError(f"{c} channels cannot be split into {cfg.groups} groups")
-    pixels = math.prod(x.shape[1:-1])
+@functools.lru_cache(maxsize=1024)
+def _sizes(shape: torch.Size, dtype: torch.dtype, param: torch.dtype, groups: int, eps: float, activation: str):
+    """(n, pixels, channels, C configuration without dropout, workspace bytes forward, backward) of a call."""
+    if len(shape) < 2:
+        raise ValueError(f"x must be [N, ..., C], got {tuple(shape)}")
+    n, pixels, c = shape[0], math.prod(shape[1:-1]), shape[-1]
+    if groups < 1 or c < 1 or c % groups:
+        raise ValueError(f"{c} channels cannot be split into {groups} groups")
     if pixels == 0:
         raise ValueError("a sample must have at least one pixel")
-    if not cfg.eps >= 0.0:
+    if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    if cfg.activation not in ACTIVATIONS:
+    if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
-    ptype = None
-    for name, t in (("weight", weight), ("bias", bias)):
+    ccfg = _lib.GroupNormCfg(groups, eps, ACTIVATIONS[activation], DTYPES[param], None)
+    need = []
+    for backward in (0, 1):
+        b = C.c_uint64()
+        _lib.check(_lib.lib().bsx_group_norm_workspace(n, pixels, c, groups, backward, C.byref(b)))
+        need.append(b.value)
+    return n, pixels, c, ccfg, *need
+
+
+def _call(x: torch.Tensor, weight, bias, cfg: GroupNormConfig):
+    """Checks what both directions share: ``_sizes``' values, weight and bias contiguous, and the C configuration."""
+    param = None
+    for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or t.shape != (c,) or t.device != x.device:
-            raise ValueError(f"{name} must be a [{c}] tensor on x's device")
-        if t.dtype not in (torch.float32, x.dtype) or t.dtype != (ptype or t.dtype):
+        if not isinstance(t, torch.Tensor) or t.shape != x.shape[-1:] or t.device != x.device:
+            raise ValueError(f"{name} must be a [{x.shape[-1]}] tensor on x's device")
+        if param is None:
+            param = t.dtype
+            if param is not torch.float32 and param is not x.dtype:
+                raise ValueError("weight and bias must both be float32 or both of x's type")
+        elif t.dtype is not param:
             raise ValueError("weight and bias must both be float32 or both of x's type")
-        ptype = t.dtype
-    drop = None
+    sizes = _sizes(x.shape, x.dtype, param or torch.float32, cfg.groups, cfg.eps, cfg.activation)
+    ccfg = sizes[3]
     if cfg.dropout is not None:
         if cfg.dropout.share != 1:
             raise ValueError("dropout in a group norm draws for each element (share 1)")
-        drop = cfg.dropout.to_c(x.device)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    ccfg = _lib.GroupNormCfg(cfg.groups, cfg.eps, ACTIVATIONS[cfg.activation], DTYPES[ptype or torch.float32],
-                             None if drop is None else C.pointer(drop))
-    return n, pixels, c, weight, bias, ccfg
-
-
-def _workspace(n: int, pixels: int, c: int, groups: int, backward: bool, device) -> torch.Tensor:
-    need = C.c_uint64()
-    _lib.check(_lib.lib().bsx_group_norm_workspace(n, pixels, c, groups, int(backward), C.byref(need)))
-    return torch.empty(need.value, dtype=torch.uint8, device=device)
+        ccfg = _lib.GroupNormCfg(ccfg.groups, ccfg.eps, ccfg.activation, ccfg.param_dtype,
+                                 C.pointer(cfg.dropout.to_c(x.device)))
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return sizes, weight, bias, ccfg
 
 
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def _empty(shape: tuple, dtype: torch.dtype, device) -> torch.Tensor:
+    """A contiguous [rows, columns] tensor: torch.empty at two thirds of its host time."""
+    return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+
+
 def group_norm_forward(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, cfg: GroupNormConfig):
     """(out, mean, rstd): out like x, mean and rstd float [N, groups] for the backward."""
     x = feature_tensor(x, "x")
-    n, pixels, c, weight, bias, ccfg = _call(x, weight, bias, cfg)
-    ctx, stream = feature_context(x.device)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, n, cfg.groups), device=x.device).unbind(0)
-    ws = _workspace(n, pixels, c, cfg.groups, False, x.device)
-    ctx.check(_lib.lib().bsx_group_norm_fwd(ctx.handle, x.data_ptr(), _ptr(weight), _ptr(bias), n, pixels, c,
-                                            DTYPES[x.dtype], C.byref(ccfg), out.data_ptr(), mean.data_ptr(),
-                                            rstd.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+    (n, pixels, c, _, need, _), weight, bias, ccfg = _call(x, weight, bias, cfg)
+    ctx, stream = feature_context(x.get_device())
+    out = torch.empty_like(x)
+    mean = _empty((n, cfg.groups), torch.float32, x.device)
+    rstd = _empty((n, cfg.groups), torch.float32, x.device)
+    ws = _empty((need, 1), torch.uint8, x.device) if need else None
+    status = _lib.lib().bsx_group_norm_fwd(ctx.handle, x.data_ptr(), _ptr(weight), _ptr(bias), n, pixels, c,
+                                           DTYPES[x.dtype], C.byref(ccfg), out.data_ptr(), mean.data_ptr(),
+                                           rstd.data_ptr(), _ptr(ws), need, stream)
+    if status:
+        ctx.check(status)
     return out, mean, rstd
 
 
@@ -91,19 +110,22 @@ def group_norm_backward(v_output: torch.Tensor, x: torch.Tensor, weight: torch.T
     an absent weight or bias is None."""
     x = feature_tensor(x, "x")
     v = like_tensor(v_output, x, "v_output")
-    n, pixels, c, weight, bias, ccfg = _call(x, weight, bias, cfg)
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        if (not isinstance(t, torch.Tensor) or t.shape != (n, cfg.groups) or t.dtype != torch.float32 or
+    (n, pixels, c, _, _, need), weight, bias, ccfg = _call(x, weight, bias, cfg)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if (not isinstance(t, torch.Tensor) or t.shape != (n, cfg.groups) or t.dtype is not torch.float32 or
                 t.device != x.device):
             raise ValueError(f"{name} must be the forward's float32 [{n}, {cfg.groups}] tensor")
-    mean, rstd = mean.contiguous(), rstd.contiguous()
-    ctx, stream = feature_context(x.device)
-    v_x = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = mean if mean.is_contiguous() else mean.contiguous()
+    rstd = rstd if rstd.is_contiguous() else rstd.contiguous()
+    ctx, stream = feature_context(x.get_device())
+    v_x = torch.empty_like(x)
     v_weight = None if weight is None else torch.empty_like(weight)
     v_bias = None if bias is None else torch.empty_like(bias)
-    ws = _workspace(n, pixels, c, cfg.groups, True, x.device)
-    ctx.check(_lib.lib().bsx_group_norm_bwd(ctx.handle, v.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias),
-                                            mean.data_ptr(), rstd.data_ptr(), n, pixels, c, DTYPES[x.dtype],
-                                            C.byref(ccfg), v_x.data_ptr(), _ptr(v_weight), _ptr(v_bias),
-                                            ws.data_ptr(), ws.numel(), stream))
+    ws = _empty((need, 1), torch.uint8, x.device) if need else None
+    status = _lib.lib().bsx_group_norm_bwd(ctx.handle, v.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias),
+                                           mean.data_ptr(), rstd.data_ptr(), n, pixels, c, DTYPES[x.dtype],
+                                           C.byref(ccfg), v_x.data_ptr(), _ptr(v_weight), _ptr(v_bias), _ptr(ws), need,
+                                           stream)
+    if status:
+        ctx.check(status)
     return v_x, v_weight, v_bias

@@ -93,7 +93,7 @@ def test_configuration_refusals(bsx_lib):
             like_tensor(t, x, "v_output")
 
     ok = bsx.GroupNormConfig(groups=4)
-    assert _call(x, None, None, ok)[:3] == (2, 3, 8)
+    assert _call(x, None, None, ok)[0][:3] == (2, 3, 8)
     half = torch.zeros(8, dtype=torch.float16)
     for bad_x, w, b, cfg in [
         (torch.zeros(8), None, None, ok),                                   # no batch
