@@ -51,7 +51,7 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 # unit keeps exact IEEE operations, because the CPU oracle (g++ -ffp-contract=off)
 # restates its decisions (culling, tile counts, alpha and early-out tests, the
 # raster backward's replay of the forward) or its results bit for bit.
-CONTRACTED = {"loss.cu", "group_norm_f32.cu", "group_norm_bf16.cu", "group_norm_f16.cu"}
+CONTRACTED = {"loss.cu"} | {f"group_norm_{d}_{t}.cu" for d in ("fwd", "bwd") for t in ("f32", "bf16", "f16")}
 
 
 def _compile(src: Path, verbose: bool) -> Path:

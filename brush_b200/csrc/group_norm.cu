@@ -18,9 +18,12 @@
 
 namespace bsx {
 namespace norm {
-extern template cudaError_t launch<float>(const Call&);
-extern template cudaError_t launch<__nv_bfloat16>(const Call&);
-extern template cudaError_t launch<__half>(const Call&);
+extern template cudaError_t launch_fwd<float>(const Call&);
+extern template cudaError_t launch_fwd<__nv_bfloat16>(const Call&);
+extern template cudaError_t launch_fwd<__half>(const Call&);
+extern template cudaError_t launch_bwd<float>(const Call&);
+extern template cudaError_t launch_bwd<__nv_bfloat16>(const Call&);
+extern template cudaError_t launch_bwd<__half>(const Call&);
 }  // namespace norm
 
 namespace {
@@ -91,7 +94,7 @@ bool plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t
 uint64_t workspace_of(const Plan& p, uint64_t n, uint32_t c, bool bwd) {
     if (p.small) return bwd ? 2ull * kMaxBlocks * c : 0;
     const uint64_t slots = (kMaxBlocks + (uint64_t)p.tiles * n) * p.gl;
-    if (!bwd) return 4 * slots;
+    if (!bwd) return 2 * slots;
     return 2 * slots + 2 * (kMaxBlocks + (uint64_t)p.tiles) * (p.tiles == 1 ? c : p.cols * p.v);
 }
 
@@ -158,9 +161,13 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
         if (all % 16 || !usable(a.pixels, a.c, v)) v = size == 2 && all % 4 == 0 && usable(a.pixels, a.c, 2) ? 2 : 1;
         Plan p;
         if (!plan_for(a.n, a.pixels, a.c, a.groups, v, bwd, p)) return fail(ctx, BSX_ERR_CAPACITY, "too many rows");
-        const Call call{&a, &p, cfg->activation, drop, a.per % v == 0, bwd, ctx->device, st};
+        a.act = cfg->activation;
+        a.dropping = drop;
+        const Call call{&a, &p, (int)(v / std::gcd(a.per, v)), ctx->device, st};
         prof_begin_on(ctx, st);
-        const cudaError_t e = dtype == BSX_F32 ? launch<float>(call) : dtype == BSX_BF16 ? launch<__nv_bfloat16>(call) : launch<__half>(call);
+        const cudaError_t e = dtype == BSX_F32    ? (bwd ? launch_bwd<float>(call) : launch_fwd<float>(call))
+                              : dtype == BSX_BF16 ? (bwd ? launch_bwd<__nv_bfloat16>(call) : launch_fwd<__nv_bfloat16>(call))
+                                                  : (bwd ? launch_bwd<__half>(call) : launch_fwd<__half>(call));
         if (e != cudaSuccess) {
             cudaGetLastError();
             return check_cuda(ctx, e, bwd ? "launch of norm_bwd_kernel" : "launch of norm_fwd_kernel");

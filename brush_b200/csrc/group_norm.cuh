@@ -47,8 +47,17 @@ struct Args {
     uint32_t c, groups, per;  // per = c / groups
     float eps;
     int param_f32;
+    int act, dropping;
     DropArgs drop;
 };
+
+// Kernels are compiled for each activation, with and without dropout (ACT, DROP), where their vectors have one or
+// two items; the rarer cuts share one that asks at run time (kAny).
+constexpr int kAny = 3;
+template <int ACT>
+__device__ __forceinline__ int act_of(const Args& a) { return ACT == kAny ? a.act : ACT; }
+template <int DROP>
+__device__ __forceinline__ bool drops(const Args& a) { return DROP == kAny ? a.dropping != 0 : DROP != 0; }
 
 // How the tensor is cut (plan_for in group_norm.cu).
 struct Plan {
@@ -62,6 +71,7 @@ struct Plan {
     uint32_t gl;         // most groups of a tile
     uint32_t per_unit;   // large samples: blocks of a (tile, sample), which take its rows in turn; or 0:
     uint32_t per_block;  // consecutive rows of a block, over tiles, samples and rows
+    uint32_t each, more; // per_unit: rows of a block; of the first `more` blocks, one more
     uint32_t pixels, pixels_last;  // of a row and of a sample's last row
     uint32_t ring;       // batches in shared memory
     uint32_t threads, blocks;
@@ -75,10 +85,10 @@ __device__ __forceinline__ float param(const void* p, int f32, uint32_t c, float
     if (!p) return without;
     return f32 ? __ldg((const float*)p + c) : to_f(((const T*)p)[c]);
 }
-// Of V channels from c on; wrap: they may run past the last channel (rows of several pixels).
+// Of V channels from c on, which may run past the last channel (rows of several pixels).
 template <class T, int V>
-__device__ __forceinline__ void params(const Args& a, const void* p, uint32_t c, bool wrap, float without, float (&to)[V]) {
-    if (V > 1 && !wrap && p && (uintptr_t)p % 16 == 0) {
+__device__ __forceinline__ void params(const Args& a, const void* p, uint32_t c, float without, float (&to)[V]) {
+    if (V > 2 && p && (uintptr_t)p % 16 == 0 && a.c % V == 0) {
         if (a.param_f32) {
             Pack<float, V> raw;
             raw.load((const float*)p + c);
@@ -117,64 +127,59 @@ __device__ __forceinline__ void add2(float& r0, float& r1, float a0, float a1, f
         : "=f"(r0), "=f"(r1)
         : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
-// r = a b + c, a b, a + b over V lanes; the operands of fewer lanes repeat.
+// r = a b + c, a b, a + b over V lanes; an operand of A values has each for V / A lanes.
 template <int V, int A, int B, int C>
 __device__ __forceinline__ void fma_v(float (&r)[V], const float (&a)[A], const float (&b)[B], const float (&c)[C]) {
     if constexpr (V == 1) r[0] = __fmaf_rn(a[0], b[0], c[0]);
     else
 #pragma unroll
         for (int j = 0; j < V; j += 2)
-            fma2(r[j], r[j + 1], a[j % A], a[(j + 1) % A], b[j % B], b[(j + 1) % B], c[j % C], c[(j + 1) % C]);
+            fma2(r[j], r[j + 1], a[j * A / V], a[(j + 1) * A / V], b[j * B / V], b[(j + 1) * B / V], c[j * C / V], c[(j + 1) * C / V]);
 }
 template <int V, int A, int B>
 __device__ __forceinline__ void mul_v(float (&r)[V], const float (&a)[A], const float (&b)[B]) {
     if constexpr (V == 1) r[0] = __fmul_rn(a[0], b[0]);
     else
 #pragma unroll
-        for (int j = 0; j < V; j += 2) mul2(r[j], r[j + 1], a[j % A], a[(j + 1) % A], b[j % B], b[(j + 1) % B]);
+        for (int j = 0; j < V; j += 2) mul2(r[j], r[j + 1], a[j * A / V], a[(j + 1) * A / V], b[j * B / V], b[(j + 1) * B / V]);
 }
 template <int V, int A, int B>
 __device__ __forceinline__ void add_v(float (&r)[V], const float (&a)[A], const float (&b)[B]) {
     if constexpr (V == 1) r[0] = __fadd_rn(a[0], b[0]);
     else
 #pragma unroll
-        for (int j = 0; j < V; j += 2) add2(r[j], r[j + 1], a[j % A], a[(j + 1) % A], b[j % B], b[(j + 1) % B]);
+        for (int j = 0; j < V; j += 2) add2(r[j], r[j + 1], a[j * A / V], a[(j + 1) * A / V], b[j * B / V], b[(j + 1) * B / V]);
 }
-// sum[j % A] += v[j] and sum[j % A] += a[j] b[j]: A partial sums.
-template <int V, int A>
-__device__ __forceinline__ void accumulate(float (&sum)[A], const float (&v)[V]) {
-    if constexpr (A == 1) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum[0] += v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; j += 2)
-            add2(sum[j % A], sum[(j + 1) % A], sum[j % A], sum[(j + 1) % A], v[j], v[j + 1]);
-    }
-}
-template <int V, int A>
-__device__ __forceinline__ void accumulate(float (&sum)[A], const float (&a)[V], const float (&b)[V]) {
-    if constexpr (A == 1) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum[0] = __fmaf_rn(a[j], b[j], sum[0]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; j += 2)
-            fma2(sum[j % A], sum[(j + 1) % A], a[j], a[j + 1], b[j], b[j + 1], sum[j % A], sum[(j + 1) % A]);
-    }
-}
-// Partial sums that keep the lanes of a pair apart.
+// Sums of V lanes into L items of V / L lanes each, the even and odd lanes of an item apart (kParts sums), so that
+// both lanes of a pair add at once.
 template <int V, int L>
-constexpr int kParts = L > 1 ? V : V > 1 ? 2 : 1;
-// One sum per item from them.
+constexpr int kParts = L == V ? V : 2 * L;
+template <int V, int L>
+__device__ constexpr int part_of(int j) { return L == V ? j : 2 * (j * L / V) + (j & 1); }
+template <int V, int L>
+__device__ __forceinline__ void accumulate(float (&sum)[kParts<V, L>], const float (&v)[V]) {
+    if constexpr (V == 1) sum[0] += v[0];
+    else
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            float &s = sum[part_of<V, L>(j)], &s2 = sum[part_of<V, L>(j + 1)];
+            add2(s, s2, s, s2, v[j], v[j + 1]);
+        }
+}
+template <int V, int L>
+__device__ __forceinline__ void accumulate(float (&sum)[kParts<V, L>], const float (&a)[V], const float (&b)[V]) {
+    if constexpr (V == 1) sum[0] = __fmaf_rn(a[0], b[0], sum[0]);
+    else
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            float &s = sum[part_of<V, L>(j)], &s2 = sum[part_of<V, L>(j + 1)];
+            fma2(s, s2, a[j], a[j + 1], b[j], b[j + 1], s, s2);
+        }
+}
 template <int V, int L>
 __device__ __forceinline__ void per_item(const float (&part)[kParts<V, L>], float (&item)[L]) {
-    if constexpr (L > 1 || V == 1) {
 #pragma unroll
-        for (int j = 0; j < L; ++j) item[j] = part[j];
-    } else {
-        item[0] = part[0] + part[1];
-    }
+    for (int j = 0; j < L; ++j) item[j] = L == V ? part[j] : part[2 * j] + part[L == V ? 0 : 2 * j + 1];
 }
 
 // The approximate exponential and reciprocal (2 and 1 ulp).
@@ -196,10 +201,10 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // 1 / a = b / (a b). Exponents are held below 60 so that the product stays finite: s is right to
 // a few units in the last place above 2^-60, and 2^-60 below.
 constexpr float kLog2e = 1.4426950408889634f, kGelu1 = 1.5957691216057308f, kGelu3 = 0.044715f;
-template <int ACT, int V>
-__device__ __forceinline__ void gates(const float (&z)[V], float (&s)[V], float (&e)[V]) {
+template <int V>
+__device__ __forceinline__ void gates(int act, const float (&z)[V], float (&s)[V], float (&e)[V]) {
     constexpr float one[1] = {1.0f};
-    if (ACT == BSX_ACT_SILU) {
+    if (act == BSX_ACT_SILU) {
         constexpr float k[1] = {-kLog2e};
         mul_v<V>(e, z, k);
     } else {
@@ -216,27 +221,29 @@ __device__ __forceinline__ void gates(const float (&z)[V], float (&s)[V], float 
     } else {
 #pragma unroll
         for (int j = 0; j < V; j += 2) {
-            const float r = rcp_fast(s[j] * s[j + 1]);
-            mul2(s[j], s[j + 1], s[j + 1], s[j], r, r);
+            const float r = rcp_fast(s[j] * s[j + 1]), other = s[j];
+            s[j] = s[j + 1] * r;
+            s[j + 1] = other * r;
         }
     }
 }
-template <int ACT, int V>
-__device__ __forceinline__ void activate(float (&z)[V]) {
-    if constexpr (ACT != BSX_ACT_NONE) {
-        float s[V], e[V];
-        gates<ACT>(z, s, e);
-        mul_v<V>(z, z, s);
-    }
+template <int V>
+__device__ __forceinline__ void activate(int act, float (&z)[V]) {
+    if (act == BSX_ACT_NONE) return;
+    float s[V], e[V];
+    gates<V>(act, z, s, e);
+    mul_v<V>(z, z, s);
 }
-// act'(z) = s + s (1 - s) z w'(z) = s (1 + e s z w'(z)): 1 - s = e s without a difference. NaN goes through z.
-template <int ACT, int V>
-__device__ __forceinline__ void slopes(float (&z)[V]) {
+// v act'(z): act'(z) = s + s (1 - s) z w'(z) = s (1 + e s z w'(z)): 1 - s = e s without a difference. NaN goes
+// through z.
+template <int V>
+__device__ __forceinline__ void back_activate(int act, float (&v)[V], float (&z)[V]) {
+    if (act == BSX_ACT_NONE) return;
     constexpr float one[1] = {1.0f};
     float s[V], e[V];
-    gates<ACT>(z, s, e);
+    gates<V>(act, z, s, e);
     mul_v<V>(e, e, s);
-    if (ACT == BSX_ACT_GELU_TANH) {
+    if (act == BSX_ACT_GELU_TANH) {
         constexpr float k1[1] = {kGelu1}, k3[1] = {3.0f * kGelu1 * kGelu3};
         float t[V];
         mul_v<V>(t, z, z);
@@ -245,6 +252,7 @@ __device__ __forceinline__ void slopes(float (&z)[V]) {
     }
     fma_v<V>(z, e, z, one);
     mul_v<V>(z, z, s);
+    mul_v<V>(v, v, z);
 }
 
 // drop for V elements from flat element `at` (V divides it, and 8).
@@ -259,7 +267,7 @@ __device__ __forceinline__ void drop_vector(const DropArgs& d, uint32_t step, ui
     }
 }
 
-// The columns and groups of a tile. Items are vectors where a vector lies in one group (L = 1), else elements.
+// The columns and groups of a tile. A vector has L items of V / L elements, each in one group.
 struct Tile {
     uint32_t cols;         // vectors in the tile's row
     uint32_t c0, c1;       // channels
@@ -299,7 +307,7 @@ __device__ __forceinline__ void group_span(const Args& a, const Tile& t, uint32_
 }
 
 // Place of an item in shared memory: with several items a thread, four words more every 32, so that threads write
-// 16 bytes at a time and the walks over copies of a channel meet other banks.
+// 16 bytes at a time and the walks over copies of a group's items meet other banks.
 template <int L>
 __device__ __forceinline__ uint32_t place(uint32_t e) { return L > 1 ? e + (e >> 5) * 4 : e; }
 template <int L>
@@ -388,36 +396,44 @@ __device__ __forceinline__ void group_sums(const Args& a, const Tile& t, const G
     }
 }
 
-// Group of the channel j places after c, relative to the tile's first.
-template <int L>
+// First channel of item j of a vector that starts at channel c.
+template <int V, int L>
 __device__ __forceinline__ uint32_t channel_at(const Args& a, uint32_t c, int j) {
-    uint32_t ch = c + j;
-    if (L > 1) while (ch >= a.c) ch -= a.c;  // rows of several pixels
+    uint32_t ch = c + j * (V / L);
+    if (j > 0) while (ch >= a.c) ch -= a.c;  // rows of several pixels
     return ch;
 }
 
 // Large samples. Rows are whole block iterations, numbered over tiles, samples ("units") and rows. A block has
-// parts of the units first ... last ("segments"): every per_unit-th row of one unit, or consecutive rows.
+// parts of the units first ... last ("segments"): every per_unit-th row of one unit (grid per_unit x units), or
+// consecutive rows (grid blocks x 1).
 struct Run {
     uint32_t first, last;
-    uint32_t w0, w1;  // consecutive rows
+    uint32_t w0, w1;  // first row of the unit, or consecutive rows
     uint32_t stride;  // rows from one to the next
 };
-__device__ __forceinline__ Run run_of(const Args& a, const Plan& p, uint32_t b) {
-    if (p.per_unit) return {b / p.per_unit, b / p.per_unit, b % p.per_unit, 0, p.per_unit};
-    const uint32_t total = p.rows * (uint32_t)a.n * p.tiles, w0 = b * p.per_block, w1 = min(w0 + p.per_block, total);
+__device__ __forceinline__ uint32_t block_id() { return blockIdx.y * gridDim.x + blockIdx.x; }
+__device__ __forceinline__ Run run_of(const Args& a, const Plan& p) {
+    if (p.per_unit) return {blockIdx.y, blockIdx.y, blockIdx.x, 0, p.per_unit};
+    const uint32_t total = p.rows * (uint32_t)a.n * p.tiles, w0 = blockIdx.x * p.per_block, w1 = min(w0 + p.per_block, total);
     return {w0 / p.rows, (w1 - 1) / p.rows, w0, w1, 1};
 }
-// Rows r0, r0 + stride, ... of unit u in a run.
-__device__ __forceinline__ void rows_of(const Plan& p, const Run& run, uint32_t u, uint32_t& r0, uint32_t& iters) {
+// Rows r0, r0 + stride, ... of unit u in a run; ends: the unit's last row among them.
+struct Rows {
+    uint32_t r0, iters;
+    bool ends;
+};
+__device__ __forceinline__ Rows rows_of(const Plan& p, const Run& run, uint32_t u) {
     if (p.per_unit) {
-        r0 = run.w0;
-        iters = (p.rows - r0 + run.stride - 1) / run.stride;
-    } else {
-        const uint32_t from = max(u * p.rows, run.w0);
-        r0 = from - u * p.rows;
-        iters = min((u + 1) * p.rows, run.w1) - from;
+        const bool extra = run.w0 < p.more;
+        return {run.w0, p.each + extra, p.more ? run.w0 + 1 == p.more : run.w0 + 1 == p.per_unit};
     }
+    const uint32_t from = max(u * p.rows, run.w0), to = min((u + 1) * p.rows, run.w1);
+    return {from - u * p.rows, to - from, to == (u + 1) * p.rows};
+}
+// Pixels of a block's part of a unit (of a tile of one pixel a row: rows).
+__device__ __forceinline__ float pixels_of(const Plan& p, const Rows& r) {
+    return (float)(r.iters - r.ends) * (float)p.pixels + (r.ends ? (float)p.pixels_last : 0.0f);
 }
 // Blocks that have rows of unit u: [b0, b1].
 __device__ __forceinline__ void runs_of_unit(const Plan& p, uint32_t u, uint32_t& b0, uint32_t& b1) {
@@ -431,23 +447,22 @@ __device__ __forceinline__ void runs_of_unit(const Plan& p, uint32_t u, uint32_t
 }
 struct Segment {
     uint32_t n, tile, c;      // sample, tile, channel of the thread's first element
-    uint32_t r0, iters, cnt;  // first row, rows, rows of this thread: it misses at most a sample's last row
-    uint64_t at;              // first element of the thread's vector in row r0
-    float pixels;
+    Rows rows;
+    uint32_t iters, cnt;      // rows; of this thread, which misses at most a sample's last row
+    uint64_t at;              // first element of the thread's vector in the first row
 };
 template <int V>
 __device__ __forceinline__ Segment segment_of(const Args& a, const Plan& p, const Run& run, uint32_t u, const Tile& t) {
     Segment s;
     s.tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n;
     s.n = u - s.tile * (uint32_t)a.n;
-    rows_of(p, run, u, s.r0, s.iters);
+    s.rows = rows_of(p, run, u);
+    s.iters = s.rows.iters;
     const uint32_t col = s.tile * p.cols + threadIdx.x;
-    const bool ends = s.r0 + (s.iters - 1) * run.stride + 1 == p.rows;
-    s.cnt = threadIdx.x < t.cols ? s.iters - (ends && col >= p.last) : 0;
-    s.at = (s.n * p.vecs + (uint64_t)s.r0 * p.rv + col) * V;
+    s.cnt = threadIdx.x < t.cols ? s.iters - (s.rows.ends && col >= p.last) : 0;
+    s.at = (s.n * p.vecs + (uint64_t)s.rows.r0 * p.rv + col) * V;
     s.c = col * V;
     if (p.tiles == 1) s.c -= p.by_c(s.c) * a.c;
-    s.pixels = (float)(s.iters - ends) * (float)p.pixels + (ends ? (float)p.pixels_last : 0.0f);
     return s;
 }
 // Batches of R rows of a run, each inside one segment.
@@ -455,9 +470,7 @@ template <int R>
 __device__ __forceinline__ uint32_t batches_of(const Plan& p, const Run& run) {
     uint32_t all = 0;
     for (uint32_t u = run.first; u <= run.last; ++u) {
-        uint32_t r0, iters;
-        rows_of(p, run, u, r0, iters);
-        all += (iters + R - 1) / R;
+        all += (rows_of(p, run, u).iters + R - 1) / R;
     }
     return all;
 }
@@ -468,14 +481,13 @@ struct Walk {
     uint64_t at;                  // element of row i
 
     __device__ __forceinline__ void unit(const Args& a, const Plan& p, const Run& run, bool last) {
-        uint32_t r0;
-        rows_of(p, run, u, r0, iters);
+        const Rows r = rows_of(p, run, u);
+        iters = r.iters;
         i = last ? (iters - 1) / R * R : 0;
         const uint32_t tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n, n = u - tile * (uint32_t)a.n;
         const uint32_t col = tile * p.cols + threadIdx.x;
-        const bool ends = r0 + (iters - 1) * run.stride + 1 == p.rows;
-        valid = threadIdx.x < p.cols && col < p.rv ? iters - (ends && col >= p.last) : 0;
-        at = (n * p.vecs + (uint64_t)(r0 + i * run.stride) * p.rv + col) * V;
+        valid = threadIdx.x < p.cols && col < p.rv ? iters - (r.ends && col >= p.last) : 0;
+        at = (n * p.vecs + (uint64_t)(r.r0 + i * run.stride) * p.rv + col) * V;
     }
     __device__ __forceinline__ void next(const Args& a, const Plan& p, const Run& run, uint64_t step) {
         i += R;
@@ -492,6 +504,17 @@ struct Walk {
         } else if (u > run.first) {
             --u;
             unit(a, p, run, true);
+        }
+    }
+    // Back to batch `to` of a run of `all`.
+    __device__ __forceinline__ void rewind(const Args& a, const Plan& p, const Run& run, uint64_t step, uint32_t all, uint32_t to) {
+        u = run.last;
+        unit(a, p, run, true);
+        if (run.first == run.last) {
+            at -= (uint64_t)(i - to * R) * step;
+            i = to * R;
+        } else {
+            for (uint32_t b = all - 1; b > to; --b) before(a, p, run, step);
         }
     }
 };
@@ -513,13 +536,12 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
-// Joins what the runs of a unit left for its tile's groups: thread (l, q) takes group q of every lanes-th run,
-// f(slot) gives the value pair, and sum[q] holds the total for all threads.
+// Joins what the blocks of a unit left for its tile's groups: thread (l, q) takes group q of every each-th block,
+// f(pair, count of values, q, s, s2) adds to its two sums, and sum[q] holds the totals for all threads.
 template <int V, class F>
-__device__ __forceinline__ void join_runs(const Args& a, const Plan& p, const Tile& t, uint32_t n,
+__device__ __forceinline__ void join_runs(const Args& a, const Plan& p, const Tile& t, uint32_t n, const float2* slots,
                                           float* part, float2* sum, F f) {
-    const uint32_t tid = threadIdx.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;
-    const uint32_t threads = blockDim.x;
+    const uint32_t tid = threadIdx.x, threads = blockDim.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;
     for (uint32_t q0 = 0; q0 < t.groups; q0 += threads) {
         const uint32_t groups = min(t.groups - q0, threads), each = threads / groups;
         const uint32_t l = tid / groups, q = q0 + tid - l * groups;
@@ -530,10 +552,25 @@ __device__ __forceinline__ void join_runs(const Args& a, const Plan& p, const Ti
             const uint32_t t1 = p.tiles == 1 ? 0 : ((grp + 1) * a.per - 1) / tile_c;
             for (uint32_t k = t0; k <= t1; ++k) {
                 const uint32_t u = k * (uint32_t)a.n + n, at = grp - (p.tiles == 1 ? 0 : p.by_per(k * tile_c));
+                const uint32_t width = p.tiles == 1 ? a.per
+                                                    : min((grp + 1) * a.per, min((k + 1) * tile_c, a.c)) - max(grp * a.per, k * tile_c);
                 uint32_t b0, b1;
                 runs_of_unit(p, u, b0, b1);
-#pragma unroll 4
-                for (uint32_t b = b0 + l; b <= b1; b += each) f((uint64_t)(b + u) * p.gl + at, q, s, s2);
+                constexpr int G = 8;  // loads in flight
+                for (uint32_t b = b0 + l; b <= b1; b += G * each) {
+                    float2 v[G];
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+                        if (b + i * each <= b1) v[i] = __ldcg(slots + (uint64_t)(b + i * each + u) * p.gl + at);
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+                        if (b + i * each <= b1) {
+                            const uint32_t bi = b + i * each;
+                            const Run run = p.per_unit ? Run{u, u, bi - b0, 0, 1}
+                                                       : Run{u, u, bi * p.per_block, bi * p.per_block + p.per_block, 1};
+                            f(v[i], pixels_of(p, rows_of(p, run, u)) * (float)width, q, s, s2);
+                        }
+                }
             }
         }
         part[tid] = s;
@@ -561,17 +598,18 @@ __device__ __forceinline__ void join_runs(const Args& a, const Plan& p, const Ti
     }
 }
 
-// Host side, one per element type (group_norm_{f32,bf16,f16}.cu). `whole`: a vector lies in one group.
+// Host side, one per element type and direction (group_norm_{fwd,bwd}_{f32,bf16,f16}.cu). items: L above.
 struct Call {
     const Args* a;
     Plan* p;
-    int act;
-    bool drop, whole, bwd;
+    int items;
     int device;
     cudaStream_t stream;
 };
 template <class T>
-cudaError_t launch(const Call& c);
+cudaError_t launch_fwd(const Call& c);
+template <class T>
+cudaError_t launch_bwd(const Call& c);
 
 }  // namespace norm
 }  // namespace bsx

@@ -12,28 +12,24 @@ struct GradLanes {
     float w[V], b[V], off[L], rstd[L];  // weight, bias, -mean rstd, rstd
 
     __device__ __forceinline__ void load(const Args& a, uint32_t c) {
-        params<T, V>(a, a.weight, c, L > 1, 1.0f, w);
-        params<T, V>(a, a.bias, c, L > 1, 0.0f, b);
+        params<T, V>(a, a.weight, c, 1.0f, w);
+        params<T, V>(a, a.bias, c, 0.0f, b);
     }
     __device__ __forceinline__ void stats(const Args& a, const Plan& p, uint64_t n, uint32_t c) {
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const uint64_t at = n * a.groups + p.by_per(channel_at<L>(a, c, j));
+            const uint64_t at = n * a.groups + p.by_per(channel_at<V, L>(a, c, j));
             off[j] = -__ldg(a.mean + at);
             rstd[j] = __ldg(a.rstd + at);
         }
     }
     // x becomes xh, v becomes dz
-    template <int ACT>
-    __device__ __forceinline__ void grads(float (&x)[V], float (&v)[V]) const {
+    __device__ __forceinline__ void grads(int act, float (&x)[V], float (&v)[V]) const {
         add_v<V>(x, x, off);
         mul_v<V>(x, x, rstd);
-        if constexpr (ACT != BSX_ACT_NONE) {
-            float z[V];
-            fma_v<V>(z, x, w, b);
-            slopes<ACT>(z);
-            mul_v<V>(v, v, z);
-        }
+        float z[V];
+        fma_v<V>(z, x, w, b);
+        back_activate<V>(act, v, z);
     }
 };
 
@@ -45,7 +41,7 @@ struct GroupGrad {
                                          const GradLanes<T, V, L>& lanes) {
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const float2 s = sum[p.by_per(channel_at<L>(g, c, j)) - t.g0];
+            const float2 s = sum[p.by_per(channel_at<V, L>(g, c, j)) - t.g0];
             s1[j] = -s.x / m * lanes.rstd[j];
             s2[j] = -s.y / m * lanes.rstd[j];
         }
@@ -128,7 +124,7 @@ __device__ __forceinline__ void join_channel(const Args& a, uint32_t c, const fl
 // Small samples: a block takes (sample, tile) pairs of one tile, x and v in registers between the sums and the
 // result. Channel sums go on over its samples and to the workspace at the end, [block of the tile][channel];
 // after a grid barrier (cooperative launch) a warp a channel adds them up.
-template <class T, int V, int L, int ACT, bool DROP>
+template <class T, int V, int L, int ACT, int DROP>
 __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;                       // [gl]
@@ -146,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
     for (int i = 0; i < kBatchBwd; ++i)
         if (active && row + i * p.k < rows) cnt = i + 1;
     const uint32_t c = p.tiles > 1 ? col * V : col * V - p.by_c(col * V) * a.c;
-    const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
+    const uint32_t dstep = drops<DROP>(a) ? drop_step(a.drop) : 0u;
     const float m = (float)(a.pixels * a.per);
     GradLanes<T, V, L> lanes;
     if (active) lanes.load(a, c);
@@ -169,13 +165,13 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
                 float x[V], v[V];
                 rx[i].get(x);
                 rv[i].get(v);
-                if (DROP) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, v);
-                lanes.template grads<ACT>(x, v);
+                if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, v);
+                lanes.grads(act_of<ACT>(a), x, v);
                 accumulate<V, V>(acc_a, v);
                 accumulate<V, V>(acc_b, v, x);
                 mul_v<V>(v, v, lanes.w);
-                accumulate<V, P>(s1, v);
-                accumulate<V, P>(s2, v, x);
+                accumulate<V, L>(s1, v);
+                accumulate<V, L>(s2, v, x);
             }
         float i1[L], i2[L];
         per_item<V, L>(s1, i1);
@@ -190,8 +186,8 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
                     float x[V], v[V];
                     rx[i].get(x);
                     rv[i].get(v);
-                    if (DROP) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, v);
-                    lanes.template grads<ACT>(x, v);
+                    if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, v);
+                    lanes.grads(act_of<ACT>(a), x, v);
                     gg.apply(x, v);
                     rx[i].set(x);
                     rx[i].store((T*)a.out + at + (uint64_t)i * step);
@@ -208,25 +204,27 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
         join_channel<T>(a, ch, ws + ch, gridDim.x / p.tiles, a.c);
 }
 
-// Large samples: runs and rings like the forward's, a ring for x and one for v. First pass: sums of dz and dz xh of
-// each channel in each segment, from which come the segment's sums of gamma dz and gamma dz xh of each group and the
-// block's sums of each channel, to the workspace. Grid barrier. Second pass, last row first: the group sums are
-// joined and v_x formed; then the channels are dealt to the warps of the grid.
-template <class T, int V, int L, int ACT, bool DROP>
+// Large samples: runs and rings like the forward's, a ring for x and one for v. First pass: a thread's sums of dz and
+// dz xh of each of its channels in a segment, from which come the segment's sums of gamma dz and gamma dz xh of each
+// group, to the workspace. While the other blocks arrive at the grid barrier, the block's sums of each channel follow.
+// Second pass, last row first: the group sums are joined and v_x formed. A second barrier, whose wait comes after that,
+// guards the channels' sums over the blocks, which are dealt to the warps of the grid.
+template <class T, int V, int L, int ACT, int DROP>
 __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
-    constexpr int R = kRowsBwd, F = kAheadBwd;
+    constexpr int P = kParts<V, L>, R = kRowsBwd, F = kAheadBwd;
     const uint32_t tid = threadIdx.x, threads = blockDim.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;
     float2* sum = (float2*)smem;            // [gl]
-    float2* chan = sum + p.gl;              // [tile_c]
+    float2* warp_sum = sum + p.gl;          // [warps]
+    float2* chan = warp_sum + kThreads / 32;  // [tile_c]
     float* part = (float*)(((uintptr_t)(chan + tile_c) + 15) & ~(uintptr_t)15);  // [2] places<V>
     Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + 2 * places<V>(threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][x, v][threads]
-    const Run run = run_of(a, p, blockIdx.x);
+    const Run run = run_of(a, p);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
-    const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
+    const uint32_t dstep = drops<DROP>(a) ? drop_step(a.drop) : 0u;
     float2* slots = (float2*)a.ws;                                                   // [(block + unit) gl + group]
-    float2* chans = slots + (uint64_t)(gridDim.x + p.tiles * (uint32_t)a.n) * p.gl;  // [(block + tile) tile_c + channel - c0]
+    float2* chans = slots + (uint64_t)(gridDim.x * gridDim.y + p.tiles * (uint32_t)a.n) * p.gl;  // [(block + tile) tile_c + channel - c0]
     const bool wanted = a.v_weight || a.v_bias;
 
     Walk<V, R> ahead;
@@ -253,10 +251,28 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
         copy_commit();
     }
     uint32_t batch = 0;
-    bool first = true;  // first segment of the block in its tile
     Tile t;
-    Segment g;
+    Segment g{};
     GradLanes<T, V, L> lanes;
+    // The block's sums of each channel of a tile, [(block + tile) tile_c + channel - c0]: a segment's are added to
+    // those of the block's segments before it.
+    uint32_t kept_tile = ~0u;
+    const auto keep_channels = [&](const float(&sa)[V], const float(&sb)[V]) {
+        if (!wanted) return;
+        channel_sums<V>(t, t.cols, sa, sb, g.cnt != 0, part, chan);
+        float2* to = chans + (uint64_t)(block_id() + g.tile) * tile_c;
+        for (uint32_t i = tid; i < t.c1 - t.c0; i += threads) {
+            float2 s = chan[i];
+            if (kept_tile == g.tile) {
+                const float2 before = to[i];
+                s.x += before.x;
+                s.y += before.y;
+            }
+            to[i] = s;
+        }
+        kept_tile = g.tile;
+    };
+    float sa[V], sb[V];
     for (uint32_t u = run.first; u <= run.last; ++u) {
         t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
         g = segment_of<V>(a, p, run, u, t);
@@ -264,14 +280,16 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             lanes.load(a, g.c);
             lanes.stats(a, p, g.n, g.c);
         }
-        float sa[V] = {}, sb[V] = {};
+        const GroupWalk walk = group_walk<V, L>(a, t, tid);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.0f;
         uint64_t at = g.at;
         const auto take = [&](const Pack<T, V>& px, const Pack<T, V>& pv, uint64_t where) {
             float fx[V], fv[V];
             px.get(fx);
             pv.get(fv);
-            if (DROP) drop_vector<V>(a.drop, dstep, where, fv);
-            lanes.template grads<ACT>(fx, fv);
+            if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, where, fv);
+            lanes.grads(act_of<ACT>(a), fx, fv);
             accumulate<V, V>(sa, fv);
             accumulate<V, V>(sb, fv, fx);
         };
@@ -295,61 +313,30 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             }
             copy_commit();
         }
-        channel_sums<V>(t, t.cols, sa, sb, g.cnt != 0, part, chan);
-        const uint32_t width = t.c1 - t.c0;
-        for (uint32_t q = tid; q < t.groups * t.lanes; q += threads) {  // lanes threads a group
-            uint32_t lo, hi;
-            group_span<V, V>(a, t, q >> t.log, lo, hi);
-            float s1 = 0.0f, s2 = 0.0f;
-            for (uint32_t i = lo + (q & (t.lanes - 1)); i < hi; i += t.lanes) {
-                const float wt = param<T>(a.weight, a.param_f32, t.c0 + i, 1.0f);
-                s1 = __fmaf_rn(wt, chan[i].x, s1);
-                s2 = __fmaf_rn(wt, chan[i].y, s2);
-            }
-            part[q] = s1;
-            part[t.groups * t.lanes + q] = s2;
+        float s1[P] = {}, s2[P] = {}, i1[L], i2[L];
+        if (g.cnt) {
+            accumulate<V, L>(s1, sa, lanes.w);
+            accumulate<V, L>(s2, sb, lanes.w);
         }
-        if (wanted) {
-            float2* to_chan = chans + (uint64_t)(blockIdx.x + g.tile) * tile_c;
-            for (uint32_t i = tid; i < width; i += threads) {
-                float2 s = chan[i];
-                if (!first) {
-                    const float2 before = to_chan[i];  // this block's own
-                    s.x += before.x;
-                    s.y += before.y;
-                }
-                to_chan[i] = s;
-            }
-        }
-        __syncthreads();
-        float2* to_slots = slots + (uint64_t)(blockIdx.x + u) * p.gl;
-        for (uint32_t q = tid; q < t.groups; q += threads) {
-            float s1 = 0.0f, s2 = 0.0f;
-            const uint32_t some = min(t.lanes, a.per);  // the other lanes had no channel
-            for (uint32_t l = 0; l < some; ++l) {
-                s1 += part[q * t.lanes + l];
-                s2 += part[(t.groups + q) * t.lanes + l];
-            }
-            to_slots[q] = make_float2(s1, s2);
-        }
-        __syncthreads();
-        first = p.tiles > 1 && (u + 1) / (uint32_t)a.n != g.tile;
+        per_item<V, L>(s1, i1);
+        per_item<V, L>(s2, i2);
+        group_sums<V, L, true>(a, t, walk, i1, i2, g.cnt != 0, part, warp_sum, sum);
+        for (uint32_t q = tid; q < t.groups; q += threads) slots[(uint64_t)(block_id() + u) * p.gl + q] = sum[q];
+        if (u != run.last) keep_channels(sa, sb);
     }
 
+    const cooperative_groups::grid_group grid = cooperative_groups::this_grid();
+    auto arrived = grid.barrier_arrive();
+    keep_channels(sa, sb);
     // What the second pass needs and no other block gives.
     const float m = (float)(a.pixels * a.per);
     const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
-    uint32_t next = all - 1;                                    // the batch that `ahead` is at
-    ahead.u = run.last;
-    ahead.unit(a, p, run, true);
-    while (next >= resident && next > 0) {
-        ahead.before(a, p, run, step);
-        --next;
-    }
+    uint32_t next = resident ? resident - 1 : 0;                // the batch that `ahead` is at
+    ahead.rewind(a, p, run, step, all, next);
     slot = (all - 1) % p.ring;
     to_slot = next % p.ring;
-
-    cooperative_groups::this_grid().sync();
+    grid.barrier_wait(std::move(arrived));
+    if (wanted) arrived = grid.barrier_arrive();
 
     for (uint32_t u = run.last;; --u) {
         if (u != run.last) {
@@ -362,8 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             __syncthreads();  // sum of the segment before is read no more
         }
         GroupGrad<T, V, L> gg;
-        join_runs<V>(a, p, t, g.n, part, sum, [&](uint64_t i, uint32_t, float& s1, float& s2) {
-            const float2 v = __ldcg(slots + i);
+        join_runs<V>(a, p, t, g.n, slots, part, sum, [&](float2 v, float, uint32_t, float& s1, float& s2) {
             s1 += v.x;
             s2 += v.y;
         });
@@ -373,8 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
             float fx[V], fv[V];
             px.get(fx);
             pv.get(fv);
-            if (DROP) drop_vector<V>(a.drop, dstep, where, fv);
-            lanes.template grads<ACT>(fx, fv);
+            if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, where, fv);
+            lanes.grads(act_of<ACT>(a), fx, fv);
             gg.apply(fx, fv);
             Pack<T, V> o;
             o.set(fx);
@@ -407,14 +393,16 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, co
         }
         if (u == run.first) break;
     }
-    if (wanted)
-        for (uint32_t ch = blockIdx.x * (threads / 32) + tid / 32; ch < a.c; ch += gridDim.x * (threads / 32)) {
+    if (wanted) {
+        grid.barrier_wait(std::move(arrived));
+        for (uint32_t ch = block_id() * (threads / 32) + tid / 32; ch < a.c; ch += gridDim.x * gridDim.y * (threads / 32)) {
             const uint32_t tile = p.tiles == 1 ? 0 : ch / tile_c, units = (uint32_t)a.n;
             uint32_t b0, b1, none;
             runs_of_unit(p, tile * units, b0, none);
             runs_of_unit(p, (tile + 1) * units - 1, none, b1);
             join_channel<T>(a, ch, chans + (uint64_t)(b0 + tile) * tile_c + (ch - tile * tile_c), b1 - b0 + 1, tile_c);
         }
+    }
 }
 
 }  // namespace norm

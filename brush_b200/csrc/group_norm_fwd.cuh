@@ -3,6 +3,8 @@
 
 #include <cooperative_groups.h>
 
+#include <utility>
+
 #include "group_norm.cuh"
 
 namespace bsx {
@@ -14,32 +16,31 @@ struct Lanes {
     float a[V], b[V], off[L];  // weight rstd, bias, -mean
 
     __device__ __forceinline__ void load(const Args& g, uint32_t c) {
-        params<T, V>(g, g.weight, c, L > 1, 1.0f, a);
-        params<T, V>(g, g.bias, c, L > 1, 0.0f, b);
+        params<T, V>(g, g.weight, c, 1.0f, a);
+        params<T, V>(g, g.bias, c, 0.0f, b);
     }
     // stat[q]: mean and rstd of the tile's group q
     __device__ __forceinline__ void fold(const Args& g, const Plan& p, const Tile& t, uint32_t c, const float2* stat) {
         float r[L];
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const float2 s = stat[p.by_per(channel_at<L>(g, c, j)) - t.g0];
+            const float2 s = stat[p.by_per(channel_at<V, L>(g, c, j)) - t.g0];
             off[j] = -s.x;
             r[j] = s.y;
         }
 #pragma unroll
-        for (int j = 0; j < V; ++j) a[j] *= r[L > 1 ? j : 0];
+        for (int j = 0; j < V; ++j) a[j] *= r[j * L / V];
     }
-    template <int ACT>
-    __device__ __forceinline__ void apply(float (&v)[V]) const {
+    __device__ __forceinline__ void apply(int act, float (&v)[V]) const {
         add_v<V>(v, v, off);  // exact for values near the mean: a large mean costs no digits
         fma_v<V>(v, v, a, b);
-        activate<ACT>(v);
+        activate<V>(act, v);
     }
 };
 
 // Small samples: one block per (sample, tile), at most kBatch vectors a thread, held in registers between
 // the sums and the result: x is read once. Mean, then the squares of the deviations from it.
-template <class T, int V, int L, int ACT, bool DROP>
+template <class T, int V, int L, int ACT, int DROP>
 __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;           // [gl]
@@ -76,12 +77,12 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
         if (i < cnt) {
             float f[V];
             raw[i].get(f);
-            accumulate<V, P>(acc, f);
+            accumulate<V, L>(acc, f);
         }
     per_item<V, L>(acc, val);
     group_sums<V, L, false>(a, t, walk, val, val, active, part, warp_sum, sum);
 #pragma unroll
-    for (int j = 0; j < L; ++j) off[j] = active ? -sum[p.by_per(channel_at<L>(a, c, j)) - t.g0].x / m : 0.0f;
+    for (int j = 0; j < L; ++j) off[j] = active ? -sum[p.by_per(channel_at<V, L>(a, c, j)) - t.g0].x / m : 0.0f;
     for (uint32_t q = tid; q < t.groups; q += blockDim.x) means[q] = sum[q].x / m;
 #pragma unroll
     for (int j = 0; j < P; ++j) acc[j] = 0.0f;
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
             float f[V];
             raw[i].get(f);
             add_v<V>(f, f, off);
-            accumulate<V, P>(acc, f, f);
+            accumulate<V, L>(acc, f, f);
         }
     per_item<V, L>(acc, val);
     group_sums<V, L, false>(a, t, walk, val, val, active, part, warp_sum, sum);
@@ -104,39 +105,40 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
     __syncthreads();
     if (cnt == 0) return;
     lanes.fold(a, p, t, c, sum);
-    const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
+    const uint32_t dstep = drops<DROP>(a) ? drop_step(a.drop) : 0u;
     T* out = (T*)a.out + at;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
         if (i < cnt) {
             float f[V];
             raw[i].get(f);
-            lanes.template apply<ACT>(f);
-            if (DROP) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, f);
+            lanes.apply(act_of<ACT>(a), f);
+            if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, f);
             raw[i].set(f);
             raw[i].store(out + (uint64_t)i * step);
         }
 }
 
-// Large samples: one cooperative launch, each block with a run of rows. Every thread copies its vectors of the
-// coming batches of rows into its own places of a ring in shared memory, kAhead batches ahead. First pass: mean and
-// sum of squared deviations of each group in each segment (from a pivot, the mean of a thread's first vectors, so
-// that no large mean cancels), to the workspace. Grid barrier. Second pass, last row first: the segments' statistics
-// are joined, and the rows are normalised out of the ring, which still holds the last ones; the others come again.
-template <class T, int V, int L, int ACT, bool DROP>
+// Large samples: one cooperative launch. Every thread copies its vectors of the block's coming batches of rows into
+// its own places of a ring in shared memory, kAhead batches ahead. First pass: mean and sum of squared deviations of
+// each group in each segment, to the workspace. Deviations are taken from a pivot, the group's mean over the block's
+// first batch, so that no large mean cancels (what the pivot is off by enters the sum of squares at most rows / kRows
+// times over). Grid barrier. Second pass, last row first: the segments' statistics are joined, and the rows are
+// normalised out of the ring, which still holds the last ones; the others come again.
+template <class T, int V, int L, int ACT, int DROP>
 __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, const Plan p) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;                       // [gl]
     float2* warp_sum = sum + p.gl;                     // [warps]
-    float2* pivot = warp_sum + kThreads / 32;          // [gl]: mean and count of the block's last segment
-    float* part = (float*)(((uintptr_t)(pivot + p.gl) + 15) & ~(uintptr_t)15);  // places<L>, two words a thread at least
+    float* pivot = (float*)(warp_sum + kThreads / 32);  // [gl]: later the mean of the block's segment
+    float* part = (float*)(((uintptr_t)(pivot + p.gl) + 15) & ~(uintptr_t)15);  // [2] places<L>
     const uint32_t tid = threadIdx.x, threads = blockDim.x;
-    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + max(places<L>(threads), 2 * threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][threads]
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + 2 * places<L>(threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][threads]
     constexpr int P = kParts<V, L>, R = kRows, F = kAhead;
-    const Run run = run_of(a, p, blockIdx.x);
+    const Run run = run_of(a, p);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
-    float4* slots = (float4*)a.ws;  // [(block + unit) gl + group]: mean, squared deviations, count
+    float2* slots = (float2*)a.ws;  // [(block + unit) gl + group]: mean, squared deviations
 
     Walk<V, R> ahead;
     ahead.u = run.first;
@@ -170,33 +172,44 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
         t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
         g = segment_of<V>(a, p, run, u, t);
         const GroupWalk walk = group_walk<V, L>(a, t, tid);
-        float off[L] = {}, acc[P] = {}, sq[P] = {};
+        float off[L], acc[P] = {}, sq[P] = {}, all_acc[P] = {}, all_sq[P] = {}, val[L], val2[L];
+        copy_wait<F - 1>();
+        {
+            const Pack<T, V>* at = ring + slot * R * threads;
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+                if (j < g.cnt) {
+                    float f[V];
+                    at[j * threads].get(f);
+                    accumulate<V, L>(acc, f);
+                }
+            per_item<V, L>(acc, val);
+            group_sums<V, L, false>(a, t, walk, val, val, g.cnt != 0, part, warp_sum, sum);
+            const Rows few = {0, min(g.iters, (uint32_t)R), g.rows.ends && g.iters <= R};
+            const float pixels = pixels_of(p, few);
+            for (uint32_t q = tid; q < t.groups; q += threads) {
+                uint32_t lo, hi;
+                group_span<V, V>(a, t, q, lo, hi);
+                // in the values' own type: differences from it have few digits, and a long sum of them rounds rarely,
+                // instead of by the same amount at each addition
+                pivot[q] = to_f(from_f<T>(sum[q].x / (pixels * (float)(hi - lo))));
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < L; ++j) off[j] = g.cnt ? -pivot[p.by_per(channel_at<V, L>(a, g.c, j)) - t.g0] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < P; ++j) acc[j] = 0.0f;
+        }
         const auto take = [&](const Pack<T, V>& v) {
             float f[V];
             v.get(f);
             add_v<V>(f, f, off);
-            accumulate<V, P>(acc, f);
-            accumulate<V, P>(sq, f, f);
+            accumulate<V, L>(acc, f);
+            accumulate<V, L>(sq, f, f);
         };
         for (uint32_t i0 = 0; i0 < g.iters; i0 += R, ++batch) {
             copy_wait<F - 1>();
             const Pack<T, V>* at = ring + slot * R * threads;
-            if (i0 == 0 && g.cnt) {
-                const uint32_t have = min(g.cnt, (uint32_t)R);
-#pragma unroll
-                for (int j = 0; j < R; ++j)
-                    if (j < have) {
-                        float f[V];
-                        at[j * threads].get(f);
-                        accumulate<V, P>(acc, f);
-                    }
-                per_item<V, L>(acc, off);
-                const float inv = -1.0f / (float)(have * (V / L));
-#pragma unroll
-                for (int j = 0; j < L; ++j) off[j] *= inv;
-#pragma unroll
-                for (int j = 0; j < P; ++j) acc[j] = 0.0f;
-            }
             if (i0 + R <= g.cnt) {
 #pragma unroll
                 for (int j = 0; j < R; ++j) take(at[j * threads]);
@@ -212,57 +225,44 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
                 to_slot = to_slot + 1 == p.ring ? 0 : to_slot + 1;
             }
             copy_commit();
-        }
-        const float cnt = (float)g.cnt * (V / L), inv = g.cnt ? 1.0f / cnt : 0.0f;
-        float mean[L], dev[L], val[L], s[L], s2[L];
-        per_item<V, L>(acc, s);
-        per_item<V, L>(sq, s2);
+            if (i0 / R % 16 == 15 || i0 + R >= g.iters) {  // sums of sums: no chain grows with the sample
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const float d = s[j] * inv;
-            mean[j] = d - off[j];
-            dev[j] = __fmaf_rn(-s[j], d, s2[j]);
-            if (dev[j] < 0.0f) dev[j] = 0.0f;  // rounding; NaN stays
-            val[j] = cnt * mean[j];
+                for (int j = 0; j < P; ++j) {
+                    all_acc[j] += acc[j];
+                    all_sq[j] += sq[j];
+                    acc[j] = sq[j] = 0.0f;
+                }
+            }
         }
-        group_sums<V, L, false>(a, t, walk, val, val, g.cnt != 0, part, warp_sum, sum);
+        per_item<V, L>(all_acc, val);
+        per_item<V, L>(all_sq, val2);
+        group_sums<V, L, true>(a, t, walk, val, val2, g.cnt != 0, part, warp_sum, sum);
+        const float pixels = pixels_of(p, g.rows);
         for (uint32_t q = tid; q < t.groups; q += threads) {
             uint32_t lo, hi;
             group_span<V, V>(a, t, q, lo, hi);
-            const float count = g.pixels * (float)(hi - lo);
-            pivot[q] = make_float2(sum[q].x / count, count);
+            const float2 s = sum[q];
+            const float d = s.x / (pixels * (float)(hi - lo));
+            float dev = __fmaf_rn(-s.x, d, s.y);
+            if (dev < 0.0f) dev = 0.0f;  // rounding; NaN stays
+            pivot[q] += d;
+            slots[(uint64_t)(block_id() + u) * p.gl + q] = make_float2(pivot[q], dev);
         }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            val[j] = 0.0f;
-            if (g.cnt) {
-                const float d = mean[j] - pivot[p.by_per(channel_at<L>(a, g.c, j)) - t.g0].x;
-                val[j] = __fmaf_rn(cnt * d, d, dev[j]);
-            }
-        }
-        group_sums<V, L, false>(a, t, walk, val, val, g.cnt != 0, part, warp_sum, sum);
-        for (uint32_t q = tid; q < t.groups; q += threads)
-            slots[(uint64_t)(blockIdx.x + u) * p.gl + q] = make_float4(pivot[q].x, sum[q].x, pivot[q].y, 0.0f);
     }
 
+    const cooperative_groups::grid_group grid = cooperative_groups::this_grid();
+    auto arrived = grid.barrier_arrive();
     // What the second pass needs and no other block gives.
-    const uint32_t dstep = DROP ? drop_step(a.drop) : 0u;
+    const uint32_t dstep = drops<DROP>(a) ? drop_step(a.drop) : 0u;
     const float m = (float)(a.pixels * a.per);
     const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
-    uint32_t next = all - 1;                                    // the batch that `ahead` is at
-    ahead.u = run.last;
-    ahead.unit(a, p, run, true);
-    while (next >= resident && next > 0) {
-        ahead.before(a, p, run, step);
-        --next;
-    }
+    uint32_t next = resident ? resident - 1 : 0;                // the batch that `ahead` is at
+    ahead.rewind(a, p, run, step, all, next);
     slot = (all - 1) % p.ring;
     to_slot = next % p.ring;
     Lanes<T, V, L> lanes;
     if (g.cnt) lanes.load(a, g.c);
-
-    cooperative_groups::this_grid().sync();
+    grid.barrier_wait(std::move(arrived));
 
     for (uint32_t u = run.last;; --u) {
         if (u != run.last) {
@@ -270,25 +270,23 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
             g = segment_of<V>(a, p, run, u, t);
             if (g.cnt) lanes.load(a, g.c);
             __syncthreads();  // sum and pivot are read no more
-            for (uint32_t q = tid; q < t.groups; q += threads)
-                pivot[q].x = __ldcg(slots + (uint64_t)(blockIdx.x + u) * p.gl + q).x;
+            for (uint32_t q = tid; q < t.groups; q += threads) pivot[q] = __ldcg(slots + (uint64_t)(block_id() + u) * p.gl + q).x;
             __syncthreads();
         }
         // Joined about a pivot, the mean of this block's own segment: its share of the values bounds how far off it is.
-        join_runs<V>(a, p, t, g.n, part, sum, [&](uint64_t i, uint32_t q, float& s, float& s2) {
-            const float4 v = __ldcg(slots + i);
-            const float d = v.x - pivot[q].x;
-            s = __fmaf_rn(v.z, d, s);
-            s2 += __fmaf_rn(v.z * d, d, v.y);
+        join_runs<V>(a, p, t, g.n, slots, part, sum, [&](float2 v, float count, uint32_t q, float& s, float& s2) {
+            const float d = v.x - pivot[q];
+            s = __fmaf_rn(count, d, s);
+            s2 += __fmaf_rn(count * d, d, v.y);
         });
         for (uint32_t q = tid; q < t.groups; q += threads) {
             const uint32_t grp = t.g0 + q;
-            const float d = sum[q].x / m, mean = pivot[q].x + d;
+            const float d = sum[q].x / m, mean = pivot[q] + d;
             float dev = __fmaf_rn(-sum[q].x, d, sum[q].y);
             if (dev < 0.0f) dev = 0.0f;
             const float rstd = 1.0f / sqrtf(dev / m + a.eps);
             sum[q] = make_float2(mean, rstd);
-            if (g.r0 == 0 && grp * a.per >= t.c0) {
+            if (g.rows.r0 == 0 && grp * a.per >= t.c0) {
                 a.mean[(uint64_t)g.n * a.groups + grp] = mean;
                 a.rstd[(uint64_t)g.n * a.groups + grp] = rstd;
             }
@@ -299,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, co
         const auto give = [&](const Pack<T, V>& v, uint64_t where) {
             float f[V];
             v.get(f);
-            lanes.template apply<ACT>(f);
-            if (DROP) drop_vector<V>(a.drop, dstep, where, f);
+            lanes.apply(act_of<ACT>(a), f);
+            if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, where, f);
             Pack<T, V> o;
             o.set(f);
             o.store((T*)a.out + where);

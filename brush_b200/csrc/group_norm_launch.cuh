@@ -28,9 +28,9 @@ cudaError_t prepare(K kernel, std::atomic<uint64_t>& done, int device) {
 }
 
 template <class K>
-cudaError_t cooperative(K kernel, const Args& a, const Plan& p, uint32_t blocks, uint32_t bytes, cudaStream_t st) {
+cudaError_t cooperative(K kernel, const Args& a, const Plan& p, dim3 blocks, uint32_t bytes, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks);
+    cfg.gridDim = blocks;
     cfg.blockDim = dim3(p.threads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = st;
@@ -42,20 +42,20 @@ cudaError_t cooperative(K kernel, const Args& a, const Plan& p, uint32_t blocks,
     return cudaLaunchKernelEx(&cfg, kernel, a, p);
 }
 
-template <class T, int V, int L, int ACT, bool DROP>
+template <class T, int V, int L, int ACT, int DROP, bool BWD>
 cudaError_t launch_one(const Call& c) {
     const Args& a = *c.a;
     Plan& p = *c.p;
     const int sms = sm_count(c.device);
     const uint32_t sums = 8 * (p.gl + kThreads / 32);  // sum, warp_sum
-    if (p.small && !c.bwd) {
+    if constexpr (!BWD) if (p.small) {
         static std::atomic<uint64_t> done{0};
         auto k = small_fwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
         k<<<p.blocks, p.threads, sums + 16 + 4 * (p.gl + places<L>(p.threads)), c.stream>>>(a, p);
         return cudaSuccess;
     }
-    if (p.small) {
+    if constexpr (BWD) if (p.small) {
         static std::atomic<uint64_t> done{0};
         auto k = small_bwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
@@ -76,56 +76,71 @@ cudaError_t launch_one(const Call& c) {
         return cooperative(k, a, p, p.blocks < most ? p.blocks : most / p.tiles * p.tiles, bytes, c.stream);
     }
     const uint32_t tile_c = p.tiles == 1 ? a.c : p.cols * V;
-    const uint32_t words = places<L>(p.threads) > 2 * p.threads ? places<L>(p.threads) : 2 * p.threads;
-    const uint32_t head = 16 + (c.bwd ? 8 * (p.gl + tile_c + places<V>(p.threads)) : sums + 8 * p.gl + 4 * words);
-    const uint32_t row = p.threads * (uint32_t)sizeof(Pack<T, V>) * (c.bwd ? 2 : 1);  // a single 16-bit element takes a word
+    const uint32_t head = 32 + sums + (BWD ? 8 * (tile_c + places<V>(p.threads)) : 4 * p.gl + 8 * places<L>(p.threads));
+    const uint32_t row = p.threads * (uint32_t)sizeof(Pack<T, V>) * (BWD ? 2 : 1);  // a single 16-bit element takes a word
     // Where units are few, each has blocks of its own, so that no block sums and joins twice; where that would
     // leave more than a tenth of the SMs idle, runs cross units.
     const uint32_t units = (uint32_t)a.n * p.tiles, total = p.rows * units;
     uint32_t blocks = total < (uint32_t)sms ? total : (uint32_t)sms;
     p.per_unit = blocks / units;
     if (p.per_unit > 0 && p.per_unit * units * 10 >= blocks * 9) {
-        p.per_block = (p.rows + p.per_unit - 1) / p.per_unit;
+        p.each = p.rows / p.per_unit;
+        p.more = p.rows % p.per_unit;
+        p.per_block = p.each + 1;
         blocks = p.per_unit * units;
     } else {
         p.per_unit = 0;
         p.per_block = (total + blocks - 1) / blocks;
         blocks = (total + p.per_block - 1) / p.per_block;
     }
-    const uint32_t rows = c.bwd ? kRowsBwd : kRows, batch = rows * row;
+    const uint32_t rows = BWD ? kRowsBwd : kRows, batch = rows * row;
     // the longest run's batches: its rows, and a cut batch at each end of a unit
     const uint32_t longest = p.per_block / rows + 1 + (p.per_unit ? 0 : p.per_block / p.rows + 1);
     p.ring = (kSharedMost - 16 - head) / batch;
     if (p.ring > longest) p.ring = longest;
     const uint32_t bytes = head + 16 + p.ring * batch;
-    if (c.bwd) {
-        static std::atomic<uint64_t> done{0};
-        auto k = large_bwd_kernel<T, V, L, ACT, DROP>;
-        if (cudaError_t e = prepare(k, done, c.device)) return e;
-        return cooperative(k, a, p, blocks, bytes, c.stream);
-    }
+    const dim3 grid = p.per_unit ? dim3(p.per_unit, units) : dim3(blocks);
     static std::atomic<uint64_t> done{0};
-    auto k = large_fwd_kernel<T, V, L, ACT, DROP>;
+    const auto k = [] {
+        if constexpr (BWD) return large_bwd_kernel<T, V, L, ACT, DROP>;
+        else return large_fwd_kernel<T, V, L, ACT, DROP>;
+    }();
     if (cudaError_t e = prepare(k, done, c.device)) return e;
-    return cooperative(k, a, p, blocks, bytes, c.stream);
+    return cooperative(k, a, p, grid, bytes, c.stream);
 }
 
-template <class T, int V, int L>
+template <class T, int V, int L, bool BWD>
 cudaError_t by_act(const Call& c) {
-    if (c.act == BSX_ACT_NONE)
-        return c.drop ? launch_one<T, V, L, BSX_ACT_NONE, true>(c) : launch_one<T, V, L, BSX_ACT_NONE, false>(c);
-    if (c.act == BSX_ACT_SILU)
-        return c.drop ? launch_one<T, V, L, BSX_ACT_SILU, true>(c) : launch_one<T, V, L, BSX_ACT_SILU, false>(c);
-    return c.drop ? launch_one<T, V, L, BSX_ACT_GELU_TANH, true>(c) : launch_one<T, V, L, BSX_ACT_GELU_TANH, false>(c);
+    const bool drop = c.a->dropping;
+    switch (c.a->act) {
+        case BSX_ACT_NONE:
+            return drop ? launch_one<T, V, L, BSX_ACT_NONE, 1, BWD>(c) : launch_one<T, V, L, BSX_ACT_NONE, 0, BWD>(c);
+        case BSX_ACT_SILU:
+            return drop ? launch_one<T, V, L, BSX_ACT_SILU, 1, BWD>(c) : launch_one<T, V, L, BSX_ACT_SILU, 0, BWD>(c);
+    }
+    return drop ? launch_one<T, V, L, BSX_ACT_GELU_TANH, 1, BWD>(c) : launch_one<T, V, L, BSX_ACT_GELU_TANH, 0, BWD>(c);
 }
 
-template <class T>
+template <class T, bool BWD>
 cudaError_t launch(const Call& c) {
-    constexpr int kMost = 16 / (int)sizeof(T);
-    if (c.p->v == kMost) return c.whole ? by_act<T, kMost, 1>(c) : by_act<T, kMost, kMost>(c);
+    constexpr int M = 16 / (int)sizeof(T);
+    if (c.p->v == M) {
+        if (c.items == 1) return by_act<T, M, 1, BWD>(c);
+        if (c.items == 2) return by_act<T, M, 2, BWD>(c);
+        if (M == 4 || c.items == 4) return launch_one<T, M, 4, kAny, kAny, BWD>(c);
+        return launch_one<T, M, M, kAny, kAny, BWD>(c);
+    }
     if constexpr (sizeof(T) == 2)
-        if (c.p->v == 2) return by_act<T, 2, 2>(c);
-    return by_act<T, 1, 1>(c);
+        if (c.p->v == 2) return launch_one<T, 2, 2, kAny, kAny, BWD>(c);
+    return launch_one<T, 1, 1, kAny, kAny, BWD>(c);
+}
+template <class T>
+cudaError_t launch_fwd(const Call& c) {
+    return launch<T, false>(c);
+}
+template <class T>
+cudaError_t launch_bwd(const Call& c) {
+    return launch<T, true>(c);
 }
 
 }  // namespace norm
