@@ -32,21 +32,22 @@ struct Div32 {
     }
 };
 
+// Kernel arguments: what the first copies need comes first, each 64 bytes of arguments being a miss of its own.
 struct Args {
     const void* x;
     const void* v;       // backward: gradient of the output
+    uint64_t n, pixels;
+    uint32_t c, groups, per;  // per = c / groups
+    int param_f32;
     const void* weight;  // null: 1
     const void* bias;    // null: 0
+    float* ws;
     void* out;           // forward: out, backward: v_x
     float* mean;
     float* rstd;
-    float* ws;
     void* v_weight;
     void* v_bias;
-    uint64_t n, pixels;
-    uint32_t c, groups, per;  // per = c / groups
     float eps;
-    int param_f32;
     int act, dropping;
     DropArgs drop;
 };
@@ -67,17 +68,17 @@ struct Plan {
     uint32_t rv;         // vectors of a row
     uint32_t cols;       // vectors of a tile's row; the last tile may have fewer
     uint32_t tiles;
-    uint32_t k;          // small samples: rows a block takes at a time
-    uint32_t gl;         // most groups of a tile
     uint32_t per_unit;   // large samples: blocks of a (tile, sample), which take its rows in turn; or 0:
     uint32_t per_block;  // consecutive rows of a block, over tiles, samples and rows
     uint32_t each, more; // per_unit: rows of a block; of the first `more` blocks, one more
-    uint32_t pixels, pixels_last;  // of a row and of a sample's last row
     uint32_t ring;       // batches in shared memory
+    uint32_t gl;         // most groups of a tile
+    uint32_t k;          // small samples: rows a block takes at a time
+    Div32 by_c, by_per, by_cols;
+    uint32_t pixels, pixels_last;  // of a row and of a sample's last row
     uint32_t threads, blocks;
     uint32_t v;          // elements of a vector
     int small;           // one block per (sample, tile), everything in registers
-    Div32 by_cols, by_per, by_c;
 };
 
 template <class T>
@@ -546,30 +547,40 @@ __device__ __forceinline__ void join_runs(const Args& a, const Plan& p, const Ti
         const uint32_t groups = min(t.groups - q0, threads), each = threads / groups;
         const uint32_t l = tid / groups, q = q0 + tid - l * groups;
         float s = 0.0f, s2 = 0.0f;
-        if (l < each) {
+        if (l < each && p.per_unit && p.tiles == 1) {  // every per_unit-th row: counts differ by one row
+            const float px = (float)p.pixels * (float)a.per, less = (float)p.each * px;
+            const uint32_t ends = p.more ? p.more - 1 : p.per_unit - 1;  // the block with the unit's last row
+            const float cut = (float)(p.pixels - p.pixels_last) * (float)a.per;
+            const float2* from = slots + (uint64_t)(n * p.per_unit + n + l) * p.gl + q;
+            constexpr int G = 4;  // loads in flight
+            for (uint32_t j = l; j < p.per_unit; j += G * each, from += (uint64_t)(G * each) * p.gl) {
+                float2 v[G];
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+                    if (j + i * each < p.per_unit) v[i] = __ldcg(from + (uint64_t)(i * each) * p.gl);
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+                    if (j + i * each < p.per_unit) {
+                        const float count = (j + i * each < p.more ? less + px : less) - (j + i * each == ends ? cut : 0.0f);
+                        f(v[i], count, q, s, s2);
+                    }
+            }
+        } else if (l < each) {
             const uint32_t grp = t.g0 + q;
             const uint32_t t0 = p.tiles == 1 ? 0 : grp * a.per / tile_c;
             const uint32_t t1 = p.tiles == 1 ? 0 : ((grp + 1) * a.per - 1) / tile_c;
+#pragma unroll 1
             for (uint32_t k = t0; k <= t1; ++k) {
                 const uint32_t u = k * (uint32_t)a.n + n, at = grp - (p.tiles == 1 ? 0 : p.by_per(k * tile_c));
                 const uint32_t width = p.tiles == 1 ? a.per
                                                     : min((grp + 1) * a.per, min((k + 1) * tile_c, a.c)) - max(grp * a.per, k * tile_c);
                 uint32_t b0, b1;
                 runs_of_unit(p, u, b0, b1);
-                constexpr int G = 8;  // loads in flight
-                for (uint32_t b = b0 + l; b <= b1; b += G * each) {
-                    float2 v[G];
-#pragma unroll
-                    for (int i = 0; i < G; ++i)
-                        if (b + i * each <= b1) v[i] = __ldcg(slots + (uint64_t)(b + i * each + u) * p.gl + at);
-#pragma unroll
-                    for (int i = 0; i < G; ++i)
-                        if (b + i * each <= b1) {
-                            const uint32_t bi = b + i * each;
-                            const Run run = p.per_unit ? Run{u, u, bi - b0, 0, 1}
-                                                       : Run{u, u, bi * p.per_block, bi * p.per_block + p.per_block, 1};
-                            f(v[i], pixels_of(p, rows_of(p, run, u)) * (float)width, q, s, s2);
-                        }
+#pragma unroll 1
+                for (uint32_t b = b0 + l; b <= b1; b += each) {
+                    const float2 v = __ldcg(slots + (uint64_t)(b + u) * p.gl + at);
+                    const Run run = p.per_unit ? Run{u, u, b - b0, 0, 1} : Run{u, u, b * p.per_block, b * p.per_block + p.per_block, 1};
+                    f(v, pixels_of(p, rows_of(p, run, u)) * (float)width, q, s, s2);
                 }
             }
         }

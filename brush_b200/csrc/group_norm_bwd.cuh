@@ -125,7 +125,7 @@ __device__ __forceinline__ void join_channel(const Args& a, uint32_t c, const fl
 // result. Channel sums go on over its samples and to the workspace at the end, [block of the tile][channel];
 // after a grid barrier (cooperative launch) a warp a channel adds them up.
 template <class T, int V, int L, int ACT, int DROP>
-__global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const Plan p) {
+__global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;                       // [gl]
     float2* warp_sum = sum + p.gl;                     // [warps]
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Args a, const
 // Second pass, last row first: the group sums are joined and v_x formed. A second barrier, whose wait comes after that,
 // guards the channels' sums over the blocks, which are dealt to the warps of the grid.
 template <class T, int V, int L, int ACT, int DROP>
-__global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Args a, const Plan p) {
+__global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
     constexpr int P = kParts<V, L>, R = kRowsBwd, F = kAheadBwd;
     const uint32_t tid = threadIdx.x, threads = blockDim.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;

@@ -41,7 +41,7 @@ struct Lanes {
 // Small samples: one block per (sample, tile), at most kBatch vectors a thread, held in registers between
 // the sums and the result: x is read once. Mean, then the squares of the deviations from it.
 template <class T, int V, int L, int ACT, int DROP>
-__global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const Plan p) {
+__global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;           // [gl]
     float2* warp_sum = sum + p.gl;         // [warps]
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Args a, const
 // times over). Grid barrier. Second pass, last row first: the segments' statistics are joined, and the rows are
 // normalised out of the ring, which still holds the last ones; the others come again.
 template <class T, int V, int L, int ACT, int DROP>
-__global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Args a, const Plan p) {
+__global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;                       // [gl]
     float2* warp_sum = sum + p.gl;                     // [warps]

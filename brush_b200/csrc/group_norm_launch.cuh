@@ -39,7 +39,7 @@ cudaError_t cooperative(K kernel, const Args& a, const Plan& p, dim3 blocks, uin
     at[0].val.cooperative = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, p);
+    return cudaLaunchKernelEx(&cfg, kernel, p, a);
 }
 
 template <class T, int V, int L, int ACT, int DROP, bool BWD>
@@ -52,7 +52,7 @@ cudaError_t launch_one(const Call& c) {
         static std::atomic<uint64_t> done{0};
         auto k = small_fwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
-        k<<<p.blocks, p.threads, sums + 16 + 4 * (p.gl + places<L>(p.threads)), c.stream>>>(a, p);
+        k<<<p.blocks, p.threads, sums + 16 + 4 * (p.gl + places<L>(p.threads)), c.stream>>>(p, a);
         return cudaSuccess;
     }
     if constexpr (BWD) if (p.small) {
