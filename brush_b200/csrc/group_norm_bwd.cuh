@@ -6,10 +6,13 @@
 namespace bsx {
 namespace norm {
 
-// What a thread needs of its V channels.
+// With d = x - mean: z = (gamma rstd) d + beta, xh = rstd d, and
+//   v_x = rstd (gamma dz - s1 - xh s2) = (gamma rstd) dz - u1 - rstd^2 u2 d,
+// u1 and u2 being the group's sums of (gamma rstd) dz and (gamma rstd) dz d over its number of values.
+// What a thread needs of its V channels:
 template <class T, int V, int L>
 struct GradLanes {
-    float w[V], b[V], off[L], rstd[L];  // weight, bias, -mean rstd, rstd
+    float w[V], b[V], off[L], rstd[L];  // gamma rstd, beta, -mean
 
     __device__ __forceinline__ void load(const Args& a, uint32_t c) {
         params<T, V>(a, a.weight, c, 1.0f, w);
@@ -23,33 +26,32 @@ struct GradLanes {
             rstd[j] = __ldg(a.rstd + at);
         }
     }
-    // x becomes xh, v becomes dz
+    __device__ __forceinline__ void scale(float (&to)[V], const float (&gamma)[V]) const { mul_v<V>(to, gamma, rstd); }
+    // x becomes d, v becomes dz
     __device__ __forceinline__ void grads(int act, float (&x)[V], float (&v)[V]) const {
         add_v<V>(x, x, off);
-        mul_v<V>(x, x, rstd);
         float z[V];
         fma_v<V>(z, x, w, b);
         back_activate<V>(act, v, z);
     }
 };
 
-// v_x = rstd (gamma dz - s1 - xh s2), s1 and s2 the group's sums over its number of values.
 template <class T, int V, int L>
 struct GroupGrad {
-    float a[V], s1[L], s2[L];  // weight rstd, -s1 rstd, -s2 rstd
+    float u1[L], u2[L];  // -u1, -rstd^2 u2
     __device__ __forceinline__ void take(const Args& g, const Plan& p, const Tile& t, uint32_t c, const float2* sum, float m,
                                          const GradLanes<T, V, L>& lanes) {
 #pragma unroll
         for (int j = 0; j < L; ++j) {
             const float2 s = sum[p.by_per(channel_at<V, L>(g, c, j)) - t.g0];
-            s1[j] = -s.x / m * lanes.rstd[j];
-            s2[j] = -s.y / m * lanes.rstd[j];
+            u1[j] = -s.x / m;
+            u2[j] = -s.y / m * lanes.rstd[j] * lanes.rstd[j];
         }
-        mul_v<V>(a, lanes.w, lanes.rstd);
     }
-    __device__ __forceinline__ void apply(float (&xh)[V], const float (&dz)[V]) const {
-        fma_v<V>(xh, xh, s2, s1);
-        fma_v<V>(xh, a, dz, xh);
+    // d becomes v_x
+    __device__ __forceinline__ void apply(const GradLanes<T, V, L>& lanes, float (&d)[V], const float (&dz)[V]) const {
+        fma_v<V>(d, d, u2, u1);
+        fma_v<V>(d, lanes.w, dz, d);
     }
 };
 
@@ -69,6 +71,7 @@ __device__ __forceinline__ void channel_sums(const Tile& t, uint32_t items, cons
         const uint32_t z = tid / width, i = tid - z * width;
         if (z < q) {
             float s = 0.0f, s2 = 0.0f;
+#pragma unroll 4
             for (uint32_t m = z; m < copies; m += q) {
                 const uint32_t at = place<V>(m * width + i);
                 s += part[at];
@@ -84,6 +87,7 @@ __device__ __forceinline__ void channel_sums(const Tile& t, uint32_t items, cons
     }
     for (uint32_t i = tid; i < width; i += blockDim.x) {
         float s = 0.0f, s2 = 0.0f;
+#pragma unroll 4
         for (uint32_t m = 0; m < q; ++m) {
             const uint32_t at = place<V>(m * width + i);
             s += part[at];
@@ -99,10 +103,16 @@ template <class T>
 __device__ __forceinline__ void join_channel(const Args& a, uint32_t c, const float2* from, uint32_t count,
                                              uint64_t stride) {
     float s = 0.0f, s2 = 0.0f;
-    for (uint32_t i = threadIdx.x & 31; i < count; i += 32) {
-        const float2 v = __ldcg(from + i * stride);
-        s += v.x;
-        s2 += v.y;
+    constexpr int G = 4;  // loads in flight
+    for (uint32_t i = threadIdx.x & 31; i < count; i += G * 32) {
+        float2 v[G];
+#pragma unroll
+        for (int k = 0; k < G; ++k) v[k] = i + k * 32 < count ? __ldcg(from + (i + k * 32) * stride) : make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+            s += v[k].x;
+            s2 += v[k].y;
+        }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
@@ -145,7 +155,10 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
     const uint32_t dstep = drops<DROP>(a) ? drop_step(a.drop) : 0u;
     const float m = (float)(a.pixels * a.per);
     GradLanes<T, V, L> lanes;
+    float gamma[V];
     if (active) lanes.load(a, c);
+#pragma unroll
+    for (int j = 0; j < V; ++j) gamma[j] = lanes.w[j];
     const GroupWalk walk = group_walk<V, L>(a, t, tid);
     float acc_a[V] = {}, acc_b[V] = {};
     for (uint32_t n = blockIdx.x / p.tiles; n < a.n; n += gridDim.x / p.tiles) {
@@ -157,7 +170,10 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
                 rx[i].load((const T*)a.x + at + (uint64_t)i * step);
                 rv[i].load((const T*)a.v + at + (uint64_t)i * step);
             }
-        if (active) lanes.stats(a, p, n, c);
+        if (active) {
+            lanes.stats(a, p, n, c);
+            lanes.scale(lanes.w, gamma);
+        }
         float s1[P] = {}, s2[P] = {};
 #pragma unroll
         for (int i = 0; i < kBatchBwd; ++i)
@@ -168,7 +184,9 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
                 if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, v);
                 lanes.grads(act_of<ACT>(a), x, v);
                 accumulate<V, V>(acc_a, v);
-                accumulate<V, V>(acc_b, v, x);
+                float t1[V];
+                mul_v<V>(t1, x, lanes.rstd);
+                accumulate<V, V>(acc_b, v, t1);
                 mul_v<V>(v, v, lanes.w);
                 accumulate<V, L>(s1, v);
                 accumulate<V, L>(s2, v, x);
@@ -188,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
                     rv[i].get(v);
                     if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, at + (uint64_t)i * step, v);
                     lanes.grads(act_of<ACT>(a), x, v);
-                    gg.apply(x, v);
+                    gg.apply(lanes, x, v);
                     rx[i].set(x);
                     rx[i].store((T*)a.out + at + (uint64_t)i * step);
                 }
@@ -205,10 +223,9 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
 }
 
 // Large samples: runs and rings like the forward's, a ring for x and one for v. First pass: a thread's sums of dz and
-// dz xh of each of its channels in a segment, from which come the segment's sums of gamma dz and gamma dz xh of each
-// group, to the workspace. While the other blocks arrive at the grid barrier, the block's sums of each channel follow.
-// Second pass, last row first: the group sums are joined and v_x formed. A second barrier, whose wait comes after that,
-// guards the channels' sums over the blocks, which are dealt to the warps of the grid.
+// dz d of each of its channels in a segment, from which come the segment's sums of each group and the block's of each
+// channel, to the workspace. Grid barrier. Second pass, last row first: the group sums are joined and v_x formed; then
+// the channels are dealt to the warps of the grid.
 template <class T, int V, int L, int ACT, int DROP>
 __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
@@ -254,24 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
     Tile t;
     Segment g{};
     GradLanes<T, V, L> lanes;
-    // The block's sums of each channel of a tile, [(block + tile) tile_c + channel - c0]: a segment's are added to
-    // those of the block's segments before it.
-    uint32_t kept_tile = ~0u;
-    const auto keep_channels = [&](const float(&sa)[V], const float(&sb)[V]) {
-        if (!wanted) return;
-        channel_sums<V>(t, t.cols, sa, sb, g.cnt != 0, part, chan);
-        float2* to = chans + (uint64_t)(block_id() + g.tile) * tile_c;
-        for (uint32_t i = tid; i < t.c1 - t.c0; i += threads) {
-            float2 s = chan[i];
-            if (kept_tile == g.tile) {
-                const float2 before = to[i];
-                s.x += before.x;
-                s.y += before.y;
-            }
-            to[i] = s;
-        }
-        kept_tile = g.tile;
-    };
+    uint32_t kept_tile = ~0u;  // the tile that the block has sums of channels for: a segment's are added to them
     float sa[V], sb[V];
     for (uint32_t u = run.first; u <= run.last; ++u) {
         t = tile_of<V, L>(a, p, p.tiles == 1 ? 0 : u / (uint32_t)a.n);
@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
         if (g.cnt) {
             lanes.load(a, g.c);
             lanes.stats(a, p, g.n, g.c);
+            lanes.scale(lanes.w, lanes.w);
         }
         const GroupWalk walk = group_walk<V, L>(a, t, tid);
 #pragma unroll
@@ -322,12 +323,25 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
         per_item<V, L>(s2, i2);
         group_sums<V, L, true>(a, t, walk, i1, i2, g.cnt != 0, part, warp_sum, sum);
         for (uint32_t q = tid; q < t.groups; q += threads) slots[(uint64_t)(block_id() + u) * p.gl + q] = sum[q];
-        if (u != run.last) keep_channels(sa, sb);
+        if (wanted) {
+            mul_v<V>(sb, sb, lanes.rstd);
+            channel_sums<V>(t, t.cols, sa, sb, g.cnt != 0, part, chan);
+            float2* to = chans + (uint64_t)(block_id() + g.tile) * tile_c;
+            for (uint32_t i = tid; i < t.c1 - t.c0; i += threads) {
+                float2 s = chan[i];
+                if (kept_tile == g.tile) {
+                    const float2 before = to[i];
+                    s.x += before.x;
+                    s.y += before.y;
+                }
+                to[i] = s;
+            }
+            kept_tile = g.tile;
+        }
     }
 
     const cooperative_groups::grid_group grid = cooperative_groups::this_grid();
     auto arrived = grid.barrier_arrive();
-    keep_channels(sa, sb);
     // What the second pass needs and no other block gives.
     const float m = (float)(a.pixels * a.per);
     const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
@@ -336,7 +350,6 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
     slot = (all - 1) % p.ring;
     to_slot = next % p.ring;
     grid.barrier_wait(std::move(arrived));
-    if (wanted) arrived = grid.barrier_arrive();
 
     for (uint32_t u = run.last;; --u) {
         if (u != run.last) {
@@ -345,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
             if (g.cnt) {
                 lanes.load(a, g.c);
                 lanes.stats(a, p, g.n, g.c);
+                lanes.scale(lanes.w, lanes.w);
             }
             __syncthreads();  // sum of the segment before is read no more
         }
@@ -361,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
             pv.get(fv);
             if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, where, fv);
             lanes.grads(act_of<ACT>(a), fx, fv);
-            gg.apply(fx, fv);
+            gg.apply(lanes, fx, fv);
             Pack<T, V> o;
             o.set(fx);
             o.store((T*)a.out + where);
@@ -394,7 +408,6 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
         if (u == run.first) break;
     }
     if (wanted) {
-        grid.barrier_wait(std::move(arrived));
         for (uint32_t ch = block_id() * (threads / 32) + tid / 32; ch < a.c; ch += gridDim.x * gridDim.y * (threads / 32)) {
             const uint32_t tile = p.tiles == 1 ? 0 : ch / tile_c, units = (uint32_t)a.n;
             uint32_t b0, b1, none;

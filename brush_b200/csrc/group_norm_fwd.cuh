@@ -41,7 +41,7 @@ struct Lanes {
 // Small samples: one block per (sample, tile), at most kBatch vectors a thread, held in registers between
 // the sums and the result: x is read once. Mean, then the squares of the deviations from it.
 template <class T, int V, int L, int ACT, int DROP>
-__global__ void __launch_bounds__(kThreads) small_fwd_kernel(const Plan p, const Args a) {
+__global__ void __launch_bounds__(kThreads, 2) small_fwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;           // [gl]
     float2* warp_sum = sum + p.gl;         // [warps]
