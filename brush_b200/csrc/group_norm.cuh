@@ -268,6 +268,37 @@ __device__ __forceinline__ void drop_vector(const DropArgs& d, uint32_t step, ui
     }
 }
 
+// Bit j: element j of a vector at flat element `at` is kept.
+template <int V>
+__device__ __forceinline__ uint32_t keep_bits(const DropArgs& d, uint32_t step, uint64_t at) {
+    return keep8(d, step, at >> 3) >> (at & 7) & ((1u << V) - 1u);
+}
+// Zeroes the dropped elements of a packed vector; the kept ones are not scaled.
+template <class T, int V>
+__device__ __forceinline__ void drop_packed(const DropArgs& d, uint32_t step, uint64_t at, Pack<T, V>& v) {
+    uint32_t keep;
+    if constexpr (V == 8) {
+        const uint32_t q0 = (uint32_t)(at >> 3), q1 = (uint32_t)(at >> 35);
+        const uint4 w = philox7(d, q0, q1, step, 0u);
+        if (!any_tie(d, w)) {
+            const uint32_t top = d.t_hi << 16 | 0xffffu, word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                v.w[k] &= (word[k] << 16 > top ? 0xffffu : 0u) | (word[k] > top ? 0xffff0000u : 0u);
+            return;
+        }
+        keep = tie_bits(d, step, q0, q1, w);
+    } else {
+        keep = keep_bits<V>(d, step, at);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (!(keep >> j & 1u)) {
+            if constexpr (sizeof(T) == 4) v.w[j] = 0u;
+            else v.w[j / 2] &= j & 1 ? 0xffffu : 0xffff0000u;
+        }
+}
+
 // The columns and groups of a tile. A vector has L items of V / L elements, each in one group.
 struct Tile {
     uint32_t cols;         // vectors in the tile's row

@@ -239,7 +239,9 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
     const Run run = run_of(a, p);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
+    const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring after the first pass
     const uint32_t dstep = drops<DROP>(a) ? drop_step(a.drop) : 0u;
+    const float scale[1] = {a.drop.scale};
     float2* slots = (float2*)a.ws;                                                   // [(block + unit) gl + group]
     float2* chans = slots + (uint64_t)(gridDim.x * gridDim.y + p.tiles * (uint32_t)a.n) * p.gl;  // [(block + tile) tile_c + channel - c0]
     const bool wanted = a.v_weight || a.v_bias;
@@ -285,18 +287,23 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
 #pragma unroll
         for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.0f;
         uint64_t at = g.at;
-        const auto take = [&](const Pack<T, V>& px, const Pack<T, V>& pv, uint64_t where) {
+        const auto take = [&](const Pack<T, V>& px, Pack<T, V>& in, uint64_t where) {
             float fx[V], fv[V];
+            Pack<T, V> pv = in;
             px.get(fx);
+            if (drops<DROP>(a)) {
+                drop_packed(a.drop, dstep, where, pv);
+                if (batch >= resident) in = pv;  // the second pass need not draw again
+            }
             pv.get(fv);
-            if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, where, fv);
+            if (drops<DROP>(a)) mul_v<V>(fv, fv, scale);
             lanes.grads(act_of<ACT>(a), fx, fv);
             accumulate<V, V>(sa, fv);
             accumulate<V, V>(sb, fv, fx);
         };
         for (uint32_t i0 = 0; i0 < g.iters; i0 += R, ++batch) {
             copy_wait<F - 1>();
-            const Pack<T, V>* have = ring + slot * 2 * R * threads;
+            Pack<T, V>* have = ring + slot * 2 * R * threads;
             if (i0 + R <= g.cnt) {
 #pragma unroll
                 for (int j = 0; j < R; ++j) take(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
@@ -344,7 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
     auto arrived = grid.barrier_arrive();
     // What the second pass needs and no other block gives.
     const float m = (float)(a.pixels * a.per);
-    const uint32_t resident = all > p.ring ? all - p.ring : 0;  // batches from here on are in the ring
     uint32_t next = resident ? resident - 1 : 0;                // the batch that `ahead` is at
     ahead.rewind(a, p, run, step, all, next);
     slot = (all - 1) % p.ring;
@@ -369,11 +375,12 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
         });
         if (g.cnt) gg.take(a, p, t, g.c, sum, m, lanes);
         uint64_t at = g.at + (g.iters - 1) / R * R * step;
-        const auto give = [&](const Pack<T, V>& px, const Pack<T, V>& pv, uint64_t where) {
+        const auto give = [&](const Pack<T, V>& px, Pack<T, V> pv, uint64_t where) {
             float fx[V], fv[V];
             px.get(fx);
+            if (drops<DROP>(a) && batch < resident) drop_packed(a.drop, dstep, where, pv);
             pv.get(fv);
-            if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, where, fv);
+            if (drops<DROP>(a)) mul_v<V>(fv, fv, scale);
             lanes.grads(act_of<ACT>(a), fx, fv);
             gg.apply(lanes, fx, fv);
             Pack<T, V> o;
