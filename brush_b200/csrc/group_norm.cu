@@ -158,7 +158,7 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
         }
         const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.v | (uintptr_t)a.out;
         uint32_t v = 16 / (uint32_t)size;
-        if (all % 16 || !usable(a.pixels, a.c, v)) v = size == 2 && all % 4 == 0 && usable(a.pixels, a.c, 2) ? 2 : 1;
+        if (all % 16 || !usable(a.pixels, a.c, v)) v = all % (2 * size) == 0 && usable(a.pixels, a.c, 2) ? 2 : 1;
         Plan p;
         if (!plan_for(a.n, a.pixels, a.c, a.groups, v, bwd, p)) return fail(ctx, BSX_ERR_CAPACITY, "too many rows");
         a.act = cfg->activation;

@@ -551,16 +551,35 @@ struct Walk {
     }
 };
 
-// Copies into a thread's own places of shared memory, which it alone reads: no barrier, only its own wait.
+// Copies into a thread's own places of shared memory, which it alone reads: no barrier, only its own wait. A copy
+// takes at least 4 bytes: of a single 16-bit element the aligned word that holds it is copied, and `read` picks its
+// half. The word's other half is read only if it belongs to the tensor too: words start inside it where the tensor
+// starts on 4 bytes (otherwise the element is loaded and stored), and a last half word is copied alone.
 template <class T, int V>
-__device__ __forceinline__ void copy_async(Pack<T, V>* to, const T* from) {
+__device__ __forceinline__ void copy_async(Pack<T, V>* to, const T* base, uint64_t at, uint64_t count) {
     constexpr int bytes = V * (int)sizeof(T);
-    if constexpr (bytes == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
-    else if constexpr (bytes >= 4)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(bytes) : "memory");
-    else
-        to->load(from);
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (bytes == 16) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(base + at) : "memory");
+    } else if constexpr (bytes >= 4) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(base + at), "n"(bytes) : "memory");
+    } else if ((uintptr_t)base % 4 == 0) {
+        const uint64_t word = at & ~(uint64_t)1;
+        const uint32_t have = word + 1 < count ? 4u : 2u;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(base + word), "r"(have) : "memory");
+    } else {
+        Pack<T, V> v;
+        v.load(base + at);
+        v.w[0] |= v.w[0] << 16;  // in both halves
+        *to = v;
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> read(const Pack<T, V>* from, uint64_t at) {
+    Pack<T, V> v = *from;
+    if constexpr (V * sizeof(T) == 2)
+        if (at & 1) v.w[0] >>= 16;
+    return v;
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>

@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
     float2* slots = (float2*)a.ws;                                                   // [(block + unit) gl + group]
     float2* chans = slots + (uint64_t)(gridDim.x * gridDim.y + p.tiles * (uint32_t)a.n) * p.gl;  // [(block + tile) tile_c + channel - c0]
     const bool wanted = a.v_weight || a.v_bias;
+    const uint64_t count = a.n * p.vecs * V;  // elements
 
     Walk<V, R> ahead;
     ahead.u = run.first;
@@ -252,12 +253,11 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
     uint32_t to_slot = 0, slot = 0;
     const auto copy = [&]() {
         Pack<T, V>* to = ring + to_slot * 2 * R * threads;
-        const T *x = (const T*)a.x + ahead.at, *v = (const T*)a.v + ahead.at;
 #pragma unroll
         for (int j = 0; j < R; ++j)
             if (ahead.i + j < ahead.valid) {
-                copy_async<T, V>(to + 2 * j * threads, x + j * step);
-                copy_async<T, V>(to + (2 * j + 1) * threads, v + j * step);
+                copy_async<T, V>(to + 2 * j * threads, (const T*)a.x, ahead.at + j * step, count);
+                copy_async<T, V>(to + (2 * j + 1) * threads, (const T*)a.v, ahead.at + j * step, count);
             }
     };
 #pragma unroll 1
@@ -287,13 +287,16 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
 #pragma unroll
         for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.0f;
         uint64_t at = g.at;
-        const auto take = [&](const Pack<T, V>& px, Pack<T, V>& in, uint64_t where) {
+        const auto take = [&](const Pack<T, V>* px, Pack<T, V>* in, uint64_t where) {
             float fx[V], fv[V];
-            Pack<T, V> pv = in;
-            px.get(fx);
+            Pack<T, V> pv = read(in, where);
+            read(px, where).get(fx);
             if (drops<DROP>(a)) {
                 drop_packed(a.drop, dstep, where, pv);
-                if (batch >= resident) in = pv;  // the second pass need not draw again
+                if (batch >= resident) {  // the second pass need not draw again
+                    if (V * sizeof(T) == 2) pv.w[0] |= pv.w[0] << 16;
+                    *in = pv;
+                }
             }
             pv.get(fv);
             if (drops<DROP>(a)) mul_v<V>(fv, fv, scale);
@@ -306,11 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
             Pack<T, V>* have = ring + slot * 2 * R * threads;
             if (i0 + R <= g.cnt) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) take(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
+                for (int j = 0; j < R; ++j) take(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) take(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
+                    if (i0 + j < g.cnt) take(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
             }
             at += R * step;
             slot = slot + 1 == p.ring ? 0 : slot + 1;
@@ -375,9 +378,10 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
         });
         if (g.cnt) gg.take(a, p, t, g.c, sum, m, lanes);
         uint64_t at = g.at + (g.iters - 1) / R * R * step;
-        const auto give = [&](const Pack<T, V>& px, Pack<T, V> pv, uint64_t where) {
+        const auto give = [&](const Pack<T, V>* px, const Pack<T, V>* in, uint64_t where) {
             float fx[V], fv[V];
-            px.get(fx);
+            Pack<T, V> pv = read(in, where);
+            read(px, where).get(fx);
             if (drops<DROP>(a) && batch < resident) drop_packed(a.drop, dstep, where, pv);
             pv.get(fv);
             if (drops<DROP>(a)) mul_v<V>(fv, fv, scale);
@@ -393,11 +397,11 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
             const Pack<T, V>* have = ring + slot * 2 * R * threads;
             if (i0 + R <= g.cnt) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) give(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
+                for (int j = 0; j < R; ++j) give(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) give(have[2 * j * threads], have[(2 * j + 1) * threads], at + j * step);
+                    if (i0 + j < g.cnt) give(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
             }
             at -= R * step;
             slot = slot == 0 ? p.ring - 1 : slot - 1;

@@ -138,6 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
     const Run run = run_of(a, p);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
+    const uint64_t count = a.n * p.vecs * V;  // elements
     float2* slots = (float2*)a.ws;  // [(block + unit) gl + group]: mean, squared deviations
 
     Walk<V, R> ahead;
@@ -146,14 +147,13 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
     uint32_t to_slot = 0, slot = 0;  // ring places of the batch to copy and of the batch at work
     const auto copy = [&]() {
         Pack<T, V>* to = ring + to_slot * R * threads;
-        const T* x = (const T*)a.x + ahead.at;
         if (ahead.i + R <= ahead.valid) {
 #pragma unroll
-            for (int j = 0; j < R; ++j) copy_async<T, V>(to + j * threads, x + j * step);
+            for (int j = 0; j < R; ++j) copy_async<T, V>(to + j * threads, (const T*)a.x, ahead.at + j * step, count);
         } else {
 #pragma unroll
             for (int j = 0; j < R; ++j)
-                if (ahead.i + j < ahead.valid) copy_async<T, V>(to + j * threads, x + j * step);
+                if (ahead.i + j < ahead.valid) copy_async<T, V>(to + j * threads, (const T*)a.x, ahead.at + j * step, count);
         }
     };
 #pragma unroll 1
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
             for (int j = 0; j < R; ++j)
                 if (j < g.cnt) {
                     float f[V];
-                    at[j * threads].get(f);
+                    read(at + j * threads, g.at + j * step).get(f);
                     accumulate<V, L>(acc, f);
                 }
             per_item<V, L>(acc, val);
@@ -212,11 +212,11 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
             const Pack<T, V>* at = ring + slot * R * threads;
             if (i0 + R <= g.cnt) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) take(at[j * threads]);
+                for (int j = 0; j < R; ++j) take(read(at + j * threads, g.at + (i0 + j) * step));
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) take(at[j * threads]);
+                    if (i0 + j < g.cnt) take(read(at + j * threads, g.at + (i0 + j) * step));
             }
             slot = slot + 1 == p.ring ? 0 : slot + 1;
             if (batch + F < all) {
@@ -309,11 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
             const Pack<T, V>* have = ring + slot * R * threads;
             if (i0 + R <= g.cnt) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) give(have[j * threads], at + j * step);
+                for (int j = 0; j < R; ++j) give(read(have + j * threads, at + j * step), at + j * step);
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) give(have[j * threads], at + j * step);
+                    if (i0 + j < g.cnt) give(read(have + j * threads, at + j * step), at + j * step);
             }
             at -= R * step;
             slot = slot == 0 ? p.ring - 1 : slot - 1;

@@ -130,8 +130,7 @@ cudaError_t launch(const Call& c) {
         if (M == 4 || c.items == 4) return launch_one<T, M, 4, kAny, kAny, BWD>(c);
         return launch_one<T, M, M, kAny, kAny, BWD>(c);
     }
-    if constexpr (sizeof(T) == 2)
-        if (c.p->v == 2) return launch_one<T, 2, 2, kAny, kAny, BWD>(c);
+    if (c.p->v == 2) return launch_one<T, 2, 2, kAny, kAny, BWD>(c);
     return launch_one<T, 1, 1, kAny, kAny, BWD>(c);
 }
 template <class T>
