@@ -347,6 +347,7 @@ SIGNATURES = {
         C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_void_p)]
     ),
     "bsx_trainer_keep_gradients": (C.c_int, [C.c_void_p, C.c_int32]),
+    "bsx_trainer_set_dropout": (C.c_int, [C.c_void_p, C.c_double, C.c_uint64]),
     "bsx_trainer_grad2d_accum": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "bsx_trainer_raster_grads": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "bsx_trainer_grad_buffers": (

@@ -21,6 +21,7 @@
 
 #include <vector>
 
+#include "dropout.cuh"
 #include "trainer.cuh"
 
 namespace bsx {
@@ -114,6 +115,19 @@ __global__ void __launch_bounds__(kStatsThreads) mean_noise_kernel(uint32_t n, c
         noise_row(nz, i, __ldg(nz.gate + i), __ldg(nz.raw_opac + i));
 }
 
+// Opacity logits of a step with splat dropout: splat i takes draw i of the mask
+// (dropout.cuh); one left out gets -inf, which the projection culls like any
+// logit that is not finite, so it renders nothing and has no gradient.
+__global__ void __launch_bounds__(kStatsThreads)
+    splat_dropout_kernel(const float* __restrict__ raw_opac, uint32_t n, const DropArgs d, float* __restrict__ out) {
+    for (uint32_t b = blockIdx.x * kStatsThreads + threadIdx.x; b < (n + 7) / 8; b += gridDim.x * kStatsThreads) {
+        const uint32_t keep = keep8(d, d.step, b), i0 = b * 8;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            if (i0 + j < n) out[i0 + j] = keep >> j & 1u ? raw_opac[i0 + j] : -INFINITY;
+    }
+}
+
 uint32_t stats_blocks(uint32_t n) { return std::min<uint32_t>((n + kStatsThreads - 1) / kStatsThreads, 148 * 8); }
 
 size_t grad_floats(uint32_t n, uint32_t c) { return (size_t)n * (11 + 3 * (size_t)c); }
@@ -189,12 +203,29 @@ bsx_loss_cfg loss_cfg_of(const bsx_train_config& c) {
 // Render -> loss -> raster backward -> projection backward, into the given gradient buffers.
 bsx_status forward_backward(bsx_trainer* tr, const bsx_camera* cam, uint32_t w, uint32_t h, const uint32_t* gt,
                             const float* transforms, const float* sh, const float* opac, float* vt, float* vs,
-                            float* vo, float* vr, int refine, float* d_loss, bsx_render_out* out,
+                            float* vo, float* vr, int refine, float* d_loss, uint32_t step, bsx_render_out* out,
                             const FusedAdam* adam = nullptr, const GradPush* push = nullptr) {
     bsx_ctx* ctx = tr->ctx;
-    bsx_status s = bsx_render_fwd(ctx, cam, w, h, transforms, sh, opac, tr->n, tr->coeffs, tr->cfg.render_mode,
-                                  BSX_PASS_BACKWARD, tr->cfg.background, out);
+    const float* step_opac = opac;
+    bsx_status s;
+    if (tr->dropout.p > 0.0 && tr->n) {
+        DropArgs d;
+        tr->dropout.step = step;
+        if (const char* why = drop_args(&tr->dropout, &d)) return fail(ctx, BSX_ERR_INVALID_ARG, why);
+        s = ensure(ctx, tr->step_opac, (size_t)tr->n * 4);
+        if (s != BSX_OK) return s;
+        prof_begin(ctx);
+        splat_dropout_kernel<<<stats_blocks((tr->n + 7) / 8), kStatsThreads, 0, ctx->stream>>>(
+            opac, tr->n, d, tr->step_opac.as<float>());
+        s = post_launch(ctx, "splat_dropout_kernel");
+        if (s != BSX_OK) return s;
+        step_opac = tr->step_opac.as<float>();
+    }
+    s = bsx_render_fwd(ctx, cam, w, h, transforms, sh, step_opac, tr->n, tr->coeffs, tr->cfg.render_mode,
+                       BSX_PASS_BACKWARD, tr->cfg.background, out);
     if (s != BSX_OK) return s;
+    // the backward reads, and the fused AdamScaled updates, the parameters: a kept splat's logit is the same in both
+    ctx->fwd.raw_opac = opac;
     s = ensure(ctx, tr->v_output, (size_t)w * h * 16);
     if (s != BSX_OK) return s;
     const bsx_loss_cfg lc = loss_cfg_of(tr->cfg);
@@ -321,7 +352,7 @@ bsx_status bsx_trainer_destroy(bsx_trainer* tr) {
     cudaSetDevice(tr->ctx->device);
     if (tr->ctx->stream) cudaStreamSynchronize(tr->ctx->stream);
     DevBuf* bufs[] = {&tr->grads, &tr->v_combined, &tr->v_output, &tr->stats, &tr->moments, &tr->moments_next,
-                      &tr->plan_keep, &tr->plan_split, &tr->plan_scratch};
+                      &tr->plan_keep, &tr->plan_split, &tr->plan_scratch, &tr->step_opac};
     for (DevBuf* b : bufs) release(tr->ctx, *b);
     if (tr->ctx->stream) cudaStreamSynchronize(tr->ctx->stream);
     delete tr;
@@ -398,7 +429,8 @@ bsx_status bsx_trainer_reserve(bsx_trainer* tr, uint32_t max_splats) {
               {&tr->moments_next, moment_floats((uint32_t)m, tr->coeffs) * 4 + 64},
               {&tr->plan_keep, (m + 1) * 4},
               {&tr->plan_split, (m + 1) * 4},
-              {&tr->plan_scratch, (m * 6 + 32) * 4}};
+              {&tr->plan_scratch, (m * 6 + 32) * 4},
+              {&tr->step_opac, tr->dropout.p > 0.0 ? m * 4 : 0}};
     for (const R& r : rs) {
         if (r.bytes <= r.b->cap) continue;
         // keep the contents of live buffers (moments, statistics) across the growth
@@ -463,6 +495,14 @@ bsx_status bsx_trainer_keep_gradients(bsx_trainer* tr, int32_t on) {
     return BSX_OK;
 }
 
+bsx_status bsx_trainer_set_dropout(bsx_trainer* tr, double p, uint64_t seed) {
+    if (!tr) return BSX_ERR_INVALID_ARG;
+    if (!(p >= 0.0 && p < 1.0)) return fail(tr->ctx, BSX_ERR_INVALID_ARG, "splat dropout must lie in [0, 1)");
+    tr->dropout.p = p;
+    tr->dropout.seed = seed;
+    return BSX_OK;
+}
+
 bsx_status bsx_train_step(bsx_trainer* tr, const bsx_camera* cam, uint32_t w, uint32_t h, const uint32_t* gt,
                           float* transforms, float* sh, float* opac, int32_t refine, float* d_loss,
                           bsx_train_stats* stats) {
@@ -505,7 +545,7 @@ bsx_status bsx_train_step(bsx_trainer* tr, const bsx_camera* cam, uint32_t w, ui
     fa.first = tr->step == 1;
     fa.keep_grads = tr->keep_grads;
     bsx_render_out out{};
-    s = forward_backward(tr, cam, w, h, gt, transforms, sh, opac, vt, vs, vo, vr, refine, d_loss, &out, &fa);
+    s = forward_backward(tr, cam, w, h, gt, transforms, sh, opac, vt, vs, vo, vr, refine, d_loss, tr->step, &out, &fa);
     if (s != BSX_OK) return s;
     s = step_epilogue(tr, refine ? vr : nullptr, out, transforms, opac, nullptr, r.lr_mean);
     if (s != BSX_OK) return s;
@@ -557,7 +597,7 @@ bsx_status bsx_train_step_dp(bsx_trainer* tr, const bsx_camera* cam, uint32_t w,
     bsx_render_out out{};
     bsx_status s = forward_backward(tr, cam, w, h, gt, sp->d_transforms[rank], sp->d_sh_coeffs[rank],
                                     sp->d_raw_opac[rank], sp->d_v_transforms[rank], sp->d_v_sh_coeffs[rank],
-                                    sp->d_v_raw_opac[rank], ex->d_refine[rank], refine, d_loss, &out, nullptr,
+                                    sp->d_v_raw_opac[rank], ex->d_refine[rank], refine, d_loss, tr->step + 1, &out, nullptr,
                                     push ? &gp : nullptr);
     if (s != BSX_OK) return s;
     const uint32_t rb = (uint32_t)((uint64_t)tr->n * rank / world), re = (uint32_t)((uint64_t)tr->n * (rank + 1) / world);

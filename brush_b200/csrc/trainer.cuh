@@ -13,6 +13,9 @@ struct bsx_trainer {
     double mean_prev = 0.0, mean_gamma = 1.0, scale_prev = 0.0, scale_gamma = 1.0;
     uint32_t dp_epoch = 0;
     int keep_grads = 0;  // bsx_train_step also writes the dense gradients
+    // splats left out of a step at random (bsx_trainer_set_dropout)
+    bsx_dropout_cfg dropout{0.0, 0, 1, nullptr, 0};
+    bsx::DevBuf step_opac;  // this step's opacity logits, -inf where a splat is left out
     // densification: the plan of the last bsx_trainer_refine_plan
     bool planned = false;
     uint32_t plan_n = 0, plan_kept = 0, plan_split_count = 0, plan_clone_count = 0, refines = 0;

@@ -30,17 +30,18 @@ class DropoutConfig:
     share: int = 1
 
     def to_c(self, device: torch.device) -> _lib.DropoutCfg:
-        p, seed, step, share = self.p, self.seed, self.step, self.share
+        p, seed, step, share = float(self.p), int(self.seed), self.step, int(self.share)
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout p must lie in [0, 1], got {p}")
         if not 0 <= seed < 1 << 64:
             raise ValueError("dropout seed must be an unsigned 64-bit number")
-        if share < 1:
+        if not 1 <= share < 1 << 64:
             raise ValueError("dropout share must be at least 1")
         if isinstance(step, torch.Tensor):
             if step.dtype not in (torch.int32, torch.uint32) or step.numel() != 1 or step.device != device:
                 raise ValueError("a dropout step tensor must be one int32 element on the tensor's device")
             return _lib.DropoutCfg(p, seed, share, step.data_ptr(), 0)
+        step = int(step)
         if not 0 <= step < 1 << 32:
             raise ValueError("dropout step must be an unsigned 32-bit number")
         return _lib.DropoutCfg(p, seed, share, None, step)

@@ -41,7 +41,7 @@ def _sizes(shape: torch.Size, dtype: torch.dtype, param: torch.dtype, groups: in
         raise ValueError("eps must not be negative")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}")
-    ccfg = _lib.GroupNormCfg(groups, eps, ACTIVATIONS[activation], DTYPES[param], None)
+    ccfg = _lib.GroupNormCfg(int(groups), float(eps), ACTIVATIONS[activation], DTYPES[param], None)
     need = []
     for backward in (0, 1):
         b = C.c_uint64()

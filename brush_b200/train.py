@@ -29,6 +29,7 @@ from ._context import context, device_view, ptr
 from .adam import AdamGroup, AdamScaled
 from .camera import Camera
 from .dist import all_gather_rows, reduce_gradients, reduce_scatter_rows, row_shard
+from .dropout import DropoutConfig, dropout_forward
 from .loss import ImageLossConfig, image_loss_fused
 from .render import render
 from .render_bwd import SplatGrads, project_bwd, rasterize_bwd
@@ -65,6 +66,10 @@ class TrainConfig:
     noise_seed: int = 42
     # keep the view-space gradient-norm sum the gradient-threshold densification rule reads
     accumulate_grad2d: bool = False
+    # probability that a splat takes no part in a step (regularisation for few views): drawn like
+    # dropout_forward's mask, one draw for a splat, from dropout_seed and the optimizer step's number
+    splat_dropout: float = 0.0
+    dropout_seed: int = 42
 
     def to_c(self, median_scale: float, render_mode: int, gather_stats: bool) -> _lib.TrainConfig:
         c = _lib.TrainConfig()
@@ -287,6 +292,9 @@ class SplatTrainer:
                                                                           self.gather_stats))
             self.native.ctx.check(_lib.lib().bsx_trainer_keep_gradients(self.native.handle,
                                                                         int(self.keep_gradients)))
+            self.native.ctx.check(_lib.lib().bsx_trainer_set_dropout(self.native.handle,
+                                                                     float(self.config.splat_dropout),
+                                                                     int(self.config.dropout_seed)))
             self.record = self.native.record()
             if self.world > 1:
                 from .peer import PeerExchange
@@ -371,7 +379,11 @@ class SplatTrainer:
     def _nccl_step(self, camera, img_size, gt_packed, splats, compute_refine_weight) -> TrainStepStats:
         self.step_count += 1
         cfg = self.config
-        out = render(camera, img_size, splats.transforms, splats.sh_coeffs, splats.raw_opacities,
+        opac = splats.raw_opacities
+        if cfg.splat_dropout > 0.0:  # a logit that is not finite is culled, and has no gradient
+            drop = DropoutConfig(p=cfg.splat_dropout, seed=cfg.dropout_seed, step=self.step_count)
+            opac = torch.where(dropout_forward(torch.ones_like(opac), drop) > 0, opac, float("-inf"))
+        out = render(camera, img_size, splats.transforms, splats.sh_coeffs, opac,
                      splats.render_mode, cfg.background_color, _lib.PASS_BACKWARD)
         ssim_w = cfg.ssim_weight
         lcfg = ImageLossConfig(l1_weight=1.0 - ssim_w, ssim_weight=-ssim_w) if ssim_w > 0 else ImageLossConfig(1.0, 0.0)

@@ -429,6 +429,12 @@ BSX_API bsx_status bsx_trainer_grad2d_accum(bsx_trainer* tr, float** d_grad2d_ac
 BSX_API bsx_status bsx_trainer_keep_gradients(bsx_trainer* tr, int32_t on);
 BSX_API bsx_status bsx_trainer_grad_buffers(bsx_trainer* tr, float** d_v_transforms, float** d_v_sh_coeffs,
                                             float** d_v_raw_opac, float** d_v_refine_weight);
+/* Splat dropout (no counterpart in the reference; off by default): in each following training step a
+ * splat takes no part with probability p, in [0, 1): it is not rendered, has no gradient and does not
+ * count as visible. Splat i takes draw i of bsx_dropout_cfg's mask for (p, seed, step), step being the
+ * number of the optimizer step, from 1; opacities are not rescaled. Ranks with the same seed leave
+ * the same splats out. */
+BSX_API bsx_status bsx_trainer_set_dropout(bsx_trainer* tr, double p, uint64_t seed);
 /* The raster-backward rows of the last step, [N, BSX_GRAD_STRIDE] by global id
  * (the input of its projection backward); valid until the next step. */
 BSX_API bsx_status bsx_trainer_raster_grads(bsx_trainer* tr, float** d_v_combined);

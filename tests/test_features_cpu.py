@@ -81,6 +81,8 @@ def test_configuration_refusals(bsx_lib):
                dict(step=torch.zeros(1)), dict(step=torch.zeros(1, dtype=torch.int64))):
         with pytest.raises(ValueError):
             bsx.DropoutConfig(**kw).to_c(dev)
+    c = bsx.DropoutConfig(p=np.float32(0.25), seed=np.int64(7), step=np.int32(3), share=np.int64(2)).to_c(dev)
+    assert (c.p, c.seed, c.step, c.share) == (0.25, 7, 3, 2)
     c = bsx.DropoutConfig(p=0.25, seed=(1 << 64) - 1, step=(1 << 32) - 1, share=3).to_c(dev)
     assert (c.p, c.seed, c.step, c.share, c.d_step) == (0.25, (1 << 64) - 1, (1 << 32) - 1, 3, None)
 

@@ -165,6 +165,10 @@ SHAPES = [  # (n, spatial, channels, groups)
     (300, (1,), 512, 32), (70, (2, 3), 40, 5), (1, (128, 129), 24, 3), (1, (5,), 2560, 32), (2, (3, 3), 4100, 2),
     (1, (211, 307), 16, 16), (3, (50, 50), 30, 10), (1, (9,), 10007, 1), (5, (1000,), 2, 2), (1, (40_000,), 3, 3),
     (2, (512, 300), 64, 8), (9, (24, 24), 192, 24),
+    # tiles of columns: whole groups in a block's registers, wide rows, one group across tiles
+    (3, (40,), 8192, 64), (1, (700,), 8192, 2), (1, (70,), 5000, 1), (2, (3,), 70_000, 7),
+    # more samples than share the blocks evenly, so that a block's rows cross samples; odd sizes among them
+    (50, (26, 20), 64, 8), (50, (27, 19), 65, 5), (33, (130, 41), 16, 8), (40, (90, 77), 6, 3),
 ]
 
 
@@ -366,6 +370,45 @@ def test_group_norm_repeats_bit_for_bit(cuda, shape):
         got = f + bsx.group_norm_backward(v, x, w, b, f[1], f[2], cfg)
         first = first or got
         assert all(torch.equal(a, c) for a, c in zip(first, got))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2, (13, 7), 32, 8), (1, (400, 90), 64, 16), (3, (201, 7), 21, 7)])
+def test_group_norm_drops_everything(cuda, dtype, shape):
+    """p = 1 leaves nothing, whatever the gradient holds, and the statistics as they are."""
+    import brush_b200 as bsx
+
+    x, w, b, v = (t.cuda() for t in _inputs(shape, dtype, "f32", 65))
+    cfg = bsx.GroupNormConfig(groups=shape[3], activation="silu", dropout=bsx.DropoutConfig(p=1.0))
+    out, mean, rstd = bsx.group_norm_forward(x, w, b, cfg)
+    plain = bsx.group_norm_forward(x, w, b, bsx.GroupNormConfig(groups=shape[3], activation="silu"))
+    assert (out == 0).all() and torch.equal(mean, plain[1]) and torch.equal(rstd, plain[2])
+    v[0] = float("nan")
+    for g in bsx.group_norm_backward(v, x, w, b, mean, rstd, cfg):
+        assert (g == 0).all()
+
+
+def test_two_graphs_at_once(cuda):
+    """Graphs of large norms, whose blocks wait for one another, replayed on two streams at the same time."""
+    import brush_b200 as bsx
+
+    shape = (2, (120, 130), 64, 8)
+    data = [[t.cuda() for t in _inputs(shape, torch.float32, "f32", 300 + 10 * k)] for k in range(2)]
+    want = [_block(bsx, *d, 1) for d in data]
+    graphs = []
+    for d in data:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = _block(bsx, *d, 1)
+        graphs.append((graph, got, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, _, s in graphs:
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, got, _), w in zip(graphs, want):
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
 
 
 def test_group_norm_empty_batch(cuda):
@@ -587,3 +630,68 @@ def test_launches_are_counted_and_profiled(cuda):
     assert ctx.launches() >= n + 2
     assert any("dropout" in k for k in prof) and any("norm" in k for k in prof)
     assert all(ms > 0 for ms, _ in prof.values())
+
+
+# ---- splat dropout in the training step ----
+
+
+@pytest.mark.parametrize("p", [0.3, 0.7])
+def test_splat_dropout_trains_the_kept_splats(cuda, bsx_lib, p):
+    """A step with splat dropout renders, and moves, exactly the splats its mask keeps: its loss and update equal
+    those of a trainer that holds only these splats; the others stay as they are."""
+    import brush_b200 as bsx
+    from brush_b200.splats import Splats, clustered_scene, orbit_camera, random_gt
+
+    full = clustered_scene(6001, 1, "cpu", seed=3)
+    w, h = 160, 96
+    cam, gt = orbit_camera(0, 3, 8.0, w, h), random_gt(h, w, 8, "cpu").cuda()
+    n = full.num_splats
+    keep = ref.mask(n, p, 77, 1)
+    g = full.to("cuda")
+    cfg = bsx.TrainConfig(mean_noise=False, splat_dropout=p, dropout_seed=77)
+    before = g.clone()
+    tr = bsx.SplatTrainer(cfg, g)
+    st = tr.step(cam, (w, h), gt, g)
+    k = keep.cuda()
+    part = Splats(before.transforms[k].contiguous(), before.sh_coeffs[k].contiguous(), before.raw_opacities[k].contiguous(),
+                  before.render_mode)
+    tr2 = bsx.SplatTrainer(bsx.TrainConfig(mean_noise=False), part)
+    # the rate of the means follows the bounds of all splats
+    tr2.median_scale = tr.median_scale
+    tr2.native.ctx.check(bsx_lib.lib().bsx_trainer_set_median_scale(tr2.native.handle, tr.median_scale))
+    st2 = tr2.step(cam, (w, h), gt, part)
+    assert st.num_visible == st2.num_visible and st.num_intersections == st2.num_intersections
+    assert torch.equal(st.loss, st2.loss)  # the same splats in the same order
+    assert torch.equal(tr.record.vis_weight.cpu() > 0, (tr.record.vis_weight.cpu() > 0) & keep)
+    for name in ("transforms", "sh_coeffs", "raw_opacities"):
+        a, b, o = getattr(g, name), getattr(part, name), getattr(before, name)
+        assert torch.equal(a[~k], o[~k])
+        # the first AdamScaled step moves a parameter by its rate times the gradient's sign: sums of gradients in
+        # another order can turn the sign only where they cancel
+        same = (a[k] - b).abs() <= 1e-6 * (1 + b.abs())
+        assert same.float().mean() >= 0.999
+        assert not torch.equal(a[k], o[k])
+    # another step leaves others out
+    st3 = tr.step(cam, (w, h), gt, g)
+    assert st3.num_visible > 0
+    tr.close(), tr2.close()
+
+
+def test_splat_dropout_refusals_and_default(cuda, bsx_lib):
+    import brush_b200 as bsx
+    from brush_b200.splats import clustered_scene
+
+    g = clustered_scene(1000, 1, "cpu", seed=3).to("cuda")
+    for p in (1.0, -0.1, float("nan")):
+        with pytest.raises(bsx.BsxError):
+            bsx.SplatTrainer(bsx.TrainConfig(splat_dropout=p), g)
+    tr = bsx.SplatTrainer(bsx.TrainConfig(), g)
+    ctx = tr.native.ctx
+    ctx.profile(True)
+    ctx.profile_reset()
+    from brush_b200.splats import orbit_camera, random_gt
+    tr.step(orbit_camera(0, 3, 8.0, 64, 64), (64, 64), random_gt(64, 64, 1, "cpu").cuda(), g)
+    names = set(ctx.profile_read())
+    ctx.profile(False)
+    assert "splat_dropout_kernel" not in names  # off by default: the step launches what it did
+    tr.close()
