@@ -131,8 +131,9 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
         a.eps = cfg->eps;
         a.param_f32 = cfg->param_dtype == BSX_F32;
         a.ws = (float*)ws;
-        const bool drop = cfg->dropout != nullptr;
-        if (drop) {
+        a.act = cfg->activation;
+        a.dropping = cfg->dropout != nullptr;
+        if (a.dropping) {
             if (const char* why = drop_args(cfg->dropout, &a.drop)) return bad(why);
             if (cfg->dropout->share != 1) return bad("dropout in a group norm draws for each element (share 1)");
         }
@@ -144,8 +145,6 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
         if (a.pixels == 0) return fail(ctx, BSX_ERR_SHAPE, "a sample must have at least one pixel");
         if (a.n && (!a.x || !a.out || (bwd && !a.v))) return bad("null tensor");
         if (a.n && (!a.mean || !a.rstd)) return bad("null mean or rstd");
-        const uint64_t need = workspace_floats(a.n, a.pixels, a.c, a.groups, bwd) * 4;
-        if (ws_bytes < need || (need && !ws)) return fail(ctx, BSX_ERR_CAPACITY, "the workspace is too small");
         DeviceScope on(ctx->device);
         const cudaStream_t st = (cudaStream_t)stream;
         if (a.n == 0) {  // no samples: parameter gradients of nothing are 0
@@ -161,8 +160,8 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
         if (all % 16 || !usable(a.pixels, a.c, v)) v = all % (2 * size) == 0 && usable(a.pixels, a.c, 2) ? 2 : 1;
         Plan p;
         if (!plan_for(a.n, a.pixels, a.c, a.groups, v, bwd, p)) return fail(ctx, BSX_ERR_CAPACITY, "too many rows");
-        a.act = cfg->activation;
-        a.dropping = drop;
+        const uint64_t need = workspace_of(p, a.n, a.c, bwd) * 4;
+        if (ws_bytes < need || (need && !ws)) return fail(ctx, BSX_ERR_CAPACITY, "the workspace is too small");
         const Call call{&a, &p, (int)(v / std::gcd(a.per, v)), ctx->device, st};
         prof_begin_on(ctx, st);
         const cudaError_t e = dtype == BSX_F32    ? (bwd ? launch_bwd<float>(call) : launch_fwd<float>(call))
