@@ -38,25 +38,33 @@ constexpr uint64_t kMaxElements = 1ull << 42;  // the grid's limit is 2^31 block
 constexpr int kMany = 4;
 constexpr uint64_t kManyFrom = 148ull * 4 * kThreads * kMany;
 
-// share > 1: the eight elements from i belong to rows m, m + 1, ... of `share` elements. One row is the
-// common case; otherwise at most five rows (share 2) in at most two blocks of draws.
+// share > 1: the eight elements from i (a multiple of 8) belong to rows m, m + 1, ... of `share` elements: to one
+// where share is a multiple of 8, to two at most from 8 on, and to five at most (share 2) below. The branches are
+// the same for a whole launch.
 __device__ __forceinline__ void drop_rows(const DropArgs& d, uint32_t step, uint64_t i, const Divisor& share,
                                           float (&v)[8]) {
     const uint64_t m = share.of(i);
-    uint64_t left = share.d - (i - m * share.d);  // elements of row m from i on
-    uint32_t keep = keep8(d, step, m >> 3) >> (m & 7);
-    if (left >= 8) {
+    if (share.d % 8 == 0) {
+        const bool all = keep1(d, step, m);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = keep & 1u ? v[j] * d.scale : 0.0f;
+        for (int j = 0; j < 8; ++j) v[j] = all ? v[j] * d.scale : 0.0f;
         return;
     }
-    const uint32_t further = share.d < 8 ? (7 - (uint32_t)left) / (uint32_t)share.d : 0;  // rows after m + 1
-    if ((m & 7) + further + 1 > 7) keep |= keep8(d, step, (m >> 3) + 1) << (8 - (m & 7));
+    const uint64_t rest = share.d - (i - m * share.d);  // elements of row m from i on
+    uint32_t left = rest < 8 ? (uint32_t)rest : 8u, keep = keep8(d, step, m >> 3) >> (m & 7);
+    if (share.d > 8) {
+        if (left < 8 && (m & 7) == 7) keep |= keep8(d, step, (m >> 3) + 1) << 1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (j < left ? keep & 1u : keep & 2u) ? v[j] * d.scale : 0.0f;
+        return;
+    }
+    const uint32_t by = (uint32_t)share.d;
+    if ((m & 7) + (7 - left) / by + 1 > 7) keep |= keep8(d, step, (m >> 3) + 1) << (8 - (m & 7));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (left == 0) {
             keep >>= 1;
-            left = share.d;
+            left = by;
         }
         --left;
         v[j] = keep & 1u ? v[j] * d.scale : 0.0f;

@@ -78,6 +78,17 @@ __device__ __forceinline__ uint32_t keep8(const DropArgs& d, uint32_t step, uint
     return keep;
 }
 
+// Draw m alone.
+__device__ __forceinline__ bool keep1(const DropArgs& d, uint32_t step, uint64_t m) {
+    const uint32_t q0 = (uint32_t)(m >> 3), q1 = (uint32_t)(m >> 35), j = (uint32_t)m & 7u;
+    const uint4 w = philox7(d, q0, q1, step, 0u);
+    const uint32_t a = j & 2 ? w.y : w.x, b = j & 2 ? w.w : w.z, h = (j & 4 ? b : a) >> (j & 1 ? 16 : 0) & 0xffffu;
+    if (h != d.t_hi) return h > d.t_hi;
+    const uint4 l = philox7(d, q0, q1, step, 1u);
+    const uint32_t c = j & 2 ? l.y : l.x, e = j & 2 ? l.w : l.z;
+    return ((j & 4 ? e : c) >> (j & 1 ? 16 : 0) & 0xffffu) >= d.t_lo;
+}
+
 // v[j] = draw 8 q + FIRST + j kept ? v[j] scale : 0. Without a tie a draw is decided by one comparison on the
 // whole word (odd draws) or on the word shifted up (even ones).
 template <int V, int FIRST = 0>
