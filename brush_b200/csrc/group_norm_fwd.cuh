@@ -39,7 +39,9 @@ struct Lanes {
 };
 
 // Small samples: one block per (sample, tile), at most kBatch vectors a thread, held in registers between
-// the sums and the result: x is read once. Mean, then the squares of the deviations from it.
+// the sums and the result: x is read once. Mean, then the squares of the deviations from it. Latency bounds it (the
+// loads, two sums of three barriers each): one 16 x 16 x 32 float sample 5.6 us, 2048 vectors of 512 f16 channels
+// 6.2 us. Two blocks of 512 threads an SM (64 registers, a few spills) against one: 6.0 and 8.1 us for the latter.
 template <class T, int V, int L, int ACT, int DROP>
 __global__ void __launch_bounds__(kThreads, 2) small_fwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
@@ -125,6 +127,12 @@ __global__ void __launch_bounds__(kThreads, 2) small_fwd_kernel(const Plan p, co
 // first batch, so that no large mean cancels (what the pivot is off by enters the sum of squares at most rows / kRows
 // times over). Grid barrier. Second pass, last row first: the segments' statistics are joined, and the rows are
 // normalised out of the ring, which still holds the last ones; the others come again.
+// A full frame of 64 bf16 channels (265 MB, larger than L2) takes 139 us: 27 MB stay in the rings, so 765 MB cross
+// DRAM, 5.5 TB/s, 84 % of the measured copy rate; read once and written once it would be 81 us. Keeping more in L2
+// (evict_last, prefetches between the passes) gave 3 % at most; deeper rings, bulk copies and other batch sizes
+// nothing. 8 x 64 x 64 x 256 (17 MB, all of it stays) takes 15.5 us against 5.1: 5 us until the last row has arrived,
+// 1 for the sums, 1.5 each for the barrier and the join, 4 for the second pass, which the special-function unit
+// bounds (three uses for two elements, four lanes a cycle and scheduler), the rest launch and prologue.
 template <class T, int V, int L, int ACT, int DROP>
 __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
