@@ -44,12 +44,16 @@ uint32_t groups_of_tile(uint32_t c, uint32_t per, uint32_t channels, uint32_t ti
     return (channels - 1) / per + 2;  // cut groups at both ends
 }
 
-// The cut for vectors of v elements; v divides a sample. False: more rows than the kernels count.
-bool plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t v, bool bwd, Plan& p) {
+// The cut for vectors of v elements; v divides a sample, or the vectors are shifted. False: more rows than the
+// kernels count.
+bool plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t v, bool bwd, bool shifted, Plan& p) {
     const uint32_t per = c / groups, batch = bwd ? kBatchBwd : kBatch;
     p = Plan{};
     p.v = v;
-    p.vecs = pixels * c / v;
+    p.elems = pixels * c;
+    p.vecs = (p.elems + v - 1) / v;
+    p.shifted = shifted;
+    p.tail = (uint32_t)(p.elems % v);
     p.by_per = Div32::of(per, c);
     p.by_c = Div32::of(c, (uint64_t)kThreads * 8);
     const uint32_t run = c / std::gcd(c, v);  // the shortest row
@@ -57,7 +61,8 @@ bool plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t
     // Small: a block holds a (sample, tile) in registers. Tiles are whole groups and at least half a sector wide.
     const auto fits = [&](uint64_t cols) { return cols <= (uint64_t)kThreads && rows <= (kThreads / cols) * batch; };
     uint64_t cols = 0;
-    if (fits(run)) {
+    if (shifted) {
+    } else if (fits(run)) {
         cols = run;
     } else if (c % v == 0) {
         const uint64_t unit = std::lcm((uint64_t)per, (uint64_t)v) / v;
@@ -82,7 +87,7 @@ bool plan_for(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, uint32_t
     p.last = (uint32_t)(p.vecs - (uint64_t)(p.rows - 1) * p.rv);
     p.tiles = (p.rv + p.cols - 1) / p.cols;
     p.pixels = p.tiles > 1 ? 1 : p.rv * v / c;
-    p.pixels_last = p.tiles > 1 ? 1 : p.last * v / c;
+    p.pixels_last = p.tiles > 1 ? 1 : (uint32_t)((p.elems - (uint64_t)(p.rows - 1) * p.rv * v) / c);
     p.threads = (p.k * p.cols + 31) / 32 * 32;
     p.blocks = p.small ? (uint32_t)(n * p.tiles) : 0;
     p.gl = groups_of_tile(c, per, p.cols * v, p.tiles);
@@ -98,19 +103,28 @@ uint64_t workspace_of(const Plan& p, uint64_t n, uint32_t c, bool bwd) {
     return 2 * slots + 2 * (kMaxBlocks + (uint64_t)p.tiles) * (p.tiles == 1 ? c : p.cols * p.v);
 }
 
-// Vectors of v elements: v divides a sample, and a row of them fits a block or has one pixel.
-bool usable(uint64_t pixels, uint32_t c, uint32_t v) {
-    return pixels * c % v == 0 && (c % v == 0 || c / std::gcd(c, v) <= (uint32_t)kThreads);
+// Vectors of v elements: a row of them fits a block or has one pixel; and v divides a sample.
+bool rows_fit(uint32_t c, uint32_t v) { return c % v == 0 || c / std::gcd(c, v) <= (uint32_t)kThreads; }
+bool usable(uint64_t pixels, uint32_t c, uint32_t v) { return pixels * c % v == 0 && rows_fit(c, v); }
+// 16-bit samples of an odd number of elements, which start off a word: shifted vectors of 8 instead of single elements
+// cost a few us of prologue and win from 2 to 3 million elements on. Measured forward / backward, bf16, silu: 2 x 100001
+// x 37 27 / 45 us against 38 / 70, 4 x 1010615 x 5 56 / 105 against 102 / 181; but 50 x 513 x 65 24 / 30 against 21 / 27,
+// and 200 x 501 x 37, above the limit, 37 / 48 against 35 / 47.
+// Pairs keep theirs (4 x 300001 x 14 41 / 65 us, shifted 48 / 88), and so does fp32 (2 x 100001 x 37 34 / 51, 33 / 58).
+bool shifts(uint64_t n, uint64_t pixels, uint32_t c) {
+    return pixels * c % 2 && n * pixels * c >= 5u << 19 && rows_fit(c, 8);
 }
 
 uint64_t workspace_floats(uint64_t n, uint64_t pixels, uint32_t c, uint32_t groups, bool bwd) {
     uint64_t most = 0;  // of the cuts that type and alignment may choose
     Plan p;
     for (uint32_t v : {8u, 4u, 2u, 1u})
-        if (usable(pixels, c, v) && plan_for(n, pixels, c, groups, v, bwd, p)) {
-            const uint64_t w = workspace_of(p, n, c, bwd);
-            if (w > most) most = w;
-        }
+        for (bool shifted : {false, true})
+            if ((shifted ? v == 8 && shifts(n, pixels, c) : usable(pixels, c, v)) &&
+                plan_for(n, pixels, c, groups, v, bwd, shifted, p)) {
+                const uint64_t w = workspace_of(p, n, c, bwd);
+                if (w > most) most = w;
+            }
     return most;
 }
 
@@ -159,7 +173,10 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
         uint32_t v = 16 / (uint32_t)size;
         if (all % 16 || !usable(a.pixels, a.c, v)) v = all % (2 * size) == 0 && usable(a.pixels, a.c, 2) ? 2 : 1;
         Plan p;
-        if (!plan_for(a.n, a.pixels, a.c, a.groups, v, bwd, p)) return fail(ctx, BSX_ERR_CAPACITY, "too many rows");
+        bool ok = plan_for(a.n, a.pixels, a.c, a.groups, v, bwd, false, p);
+        if (size == 2 && all % 16 == 0 && !p.small && shifts(a.n, a.pixels, a.c))
+            ok = plan_for(a.n, a.pixels, a.c, a.groups, v = 8, bwd, true, p);
+        if (!ok) return fail(ctx, BSX_ERR_CAPACITY, "too many rows");
         const uint64_t need = workspace_of(p, a.n, a.c, bwd) * 4;
         if (ws_bytes < need || (need && !ws)) return fail(ctx, BSX_ERR_CAPACITY, "the workspace is too small");
         const Call call{&a, &p, (int)(v / std::gcd(a.per, v)), ctx->device, st};

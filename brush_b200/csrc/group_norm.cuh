@@ -17,9 +17,10 @@ namespace norm {
 
 constexpr int kThreads = 512;         // most threads of a block
 constexpr int kBatch = 8;             // vectors a thread holds, small samples
-constexpr int kRows = 4, kAhead = 2;  // large samples: rows of a batch, batches in flight ahead of the one at work
-constexpr int kBatchBwd = 4;          // the same for the backward, of x and of v each
-constexpr int kRowsBwd = 2, kAheadBwd = 3;
+constexpr int kBatchBwd = 4;          // of x and of v each, backward
+// Large samples: rows of a batch, and batches in flight ahead of the one at work; shifted: see Shifted samples below.
+__host__ __device__ constexpr int rows_of_batch(bool bwd, bool shifted) { return (bwd ? 2 : 4) / (shifted ? 2 : 1); }
+__host__ __device__ constexpr int batches_ahead(bool bwd, bool shifted) { return bwd == shifted ? 2 : 3; }
 constexpr uint32_t kMaxBlocks = 512;  // most blocks of a kernel that leaves partial sums
 
 // Division of x by d for x d < 2^32: with f = (2^32 + e) / d, 0 < e <= d, the product's high word is
@@ -62,6 +63,7 @@ __device__ __forceinline__ bool drops(const Args& a) { return DROP == kAny ? a.d
 
 // How the tensor is cut (plan_for in group_norm.cu).
 struct Plan {
+    uint64_t elems;      // elements of a sample
     uint64_t vecs;       // vectors of a sample
     uint32_t rows;       // rows of a sample
     uint32_t last;       // vectors of its last row
@@ -78,6 +80,8 @@ struct Plan {
     uint32_t pixels, pixels_last;  // of a row and of a sample's last row
     uint32_t threads, blocks;
     uint32_t v;          // elements of a vector
+    uint32_t tail;       // shifted: elements of a sample's last vector where it is not whole, else 0
+    int shifted;
     int small;           // one block per (sample, tile), everything in registers
 };
 
@@ -256,28 +260,30 @@ __device__ __forceinline__ void back_activate(int act, float (&v)[V], float (&z)
     mul_v<V>(v, v, z);
 }
 
-// drop for V elements from flat element `at` (V divides it, and 8).
+// Bit j: element j of a vector at flat element `at` is kept; a vector may lie across two blocks of draws.
 template <int V>
+__device__ __forceinline__ uint32_t keep_bits(const DropArgs& d, uint32_t step, uint64_t at) {
+    uint32_t keep = keep8(d, step, at >> 3) >> (at & 7);
+    if ((at & 7) + V > 8) keep |= keep8(d, step, (at >> 3) + 1) << (8 - (at & 7));
+    return keep & ((1u << V) - 1u);
+}
+// drop for V elements from flat element `at`, a multiple of V unless the sample is shifted (S).
+template <int V, bool S = false>
 __device__ __forceinline__ void drop_vector(const DropArgs& d, uint32_t step, uint64_t at, float (&v)[V]) {
-    if constexpr (V == 8) {
+    if constexpr (V == 8 && !S) {
         drop_values<8>(d, step, at >> 3, v);
     } else {
-        const uint32_t keep = keep8(d, step, at >> 3) >> (at & 7);
+        const uint32_t keep = keep_bits<V>(d, step, at);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = keep >> j & 1u ? v[j] * d.scale : 0.0f;
     }
 }
 
-// Bit j: element j of a vector at flat element `at` is kept.
-template <int V>
-__device__ __forceinline__ uint32_t keep_bits(const DropArgs& d, uint32_t step, uint64_t at) {
-    return keep8(d, step, at >> 3) >> (at & 7) & ((1u << V) - 1u);
-}
 // Zeroes the dropped elements of a packed vector; the kept ones are not scaled.
-template <class T, int V>
+template <bool S, class T, int V>
 __device__ __forceinline__ void drop_packed(const DropArgs& d, uint32_t step, uint64_t at, Pack<T, V>& v) {
     uint32_t keep;
-    if constexpr (V == 8) {
+    if constexpr (V == 8 && !S) {
         const uint32_t q0 = (uint32_t)(at >> 3), q1 = (uint32_t)(at >> 35);
         const uint4 w = philox7(d, q0, q1, step, 0u);
         if (!any_tie(d, w)) {
@@ -481,6 +487,7 @@ struct Segment {
     uint32_t n, tile, c;      // sample, tile, channel of the thread's first element
     Rows rows;
     uint32_t iters, cnt;      // rows; of this thread, which misses at most a sample's last row
+    uint32_t tail;            // shifted: the row, from 1, whose vector of this thread has p.tail elements; 0: none
     uint64_t at;              // first element of the thread's vector in the first row
 };
 template <int V>
@@ -492,7 +499,8 @@ __device__ __forceinline__ Segment segment_of(const Args& a, const Plan& p, cons
     s.iters = s.rows.iters;
     const uint32_t col = s.tile * p.cols + threadIdx.x;
     s.cnt = threadIdx.x < t.cols ? s.iters - (s.rows.ends && col >= p.last) : 0;
-    s.at = (s.n * p.vecs + (uint64_t)s.rows.r0 * p.rv + col) * V;
+    s.at = s.n * p.elems + ((uint64_t)s.rows.r0 * p.rv + col) * V;
+    s.tail = p.tail && s.rows.ends && col + 1 == p.last ? s.iters : 0;
     s.c = col * V;
     if (p.tiles == 1) s.c -= p.by_c(s.c) * a.c;
     return s;
@@ -519,7 +527,7 @@ struct Walk {
         const uint32_t tile = p.tiles == 1 ? 0 : u / (uint32_t)a.n, n = u - tile * (uint32_t)a.n;
         const uint32_t col = tile * p.cols + threadIdx.x;
         valid = threadIdx.x < p.cols && col < p.rv ? iters - (r.ends && col >= p.last) : 0;
-        at = (n * p.vecs + (uint64_t)(r.r0 + i * run.stride) * p.rv + col) * V;
+        at = n * p.elems + ((uint64_t)(r.r0 + i * run.stride) * p.rv + col) * V;
     }
     __device__ __forceinline__ void next(const Args& a, const Plan& p, const Run& run, uint64_t step) {
         i += R;
@@ -581,6 +589,91 @@ __device__ __forceinline__ Pack<T, V> read(const Pack<T, V>* from, uint64_t at) 
         if (at & 1) v.w[0] >>= 16;
     return v;
 }
+
+// Shifted samples (16-bit types, an odd number of elements): samples after the first start off a vector, or a word.
+// Their vectors are still counted from the sample's own start, so that channels, rows and pixels fall as they do
+// elsewhere, but lie across two aligned ones: a thread copies both, takes its elements out of the two, and passes
+// what reaches into the next aligned vector to its neighbour when it stores. The last vector may have fewer elements.
+// What that buys was measured where it is chosen (shifts in group_norm.cu).
+
+// V elements of two neighbouring aligned vectors from element `off` (< V) on.
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> across(const Pack<T, V>& lo, const Pack<T, V>& hi, uint32_t off) {
+    const uint32_t bytes = off * (uint32_t)sizeof(T), odd = bytes & 2u;
+    Pack<T, V> r;
+    const auto take = [&](const uint32_t(&w)[5]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r.w[k] = odd ? __funnelshift_r(w[k], w[k + 1], 16) : w[k];
+    };
+    switch (bytes >> 2) {  // the same for a whole row
+        case 0: take({lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0]}); break;
+        case 1: take({lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1]}); break;
+        case 2: take({lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2]}); break;
+        default: take({lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]}); break;
+    }
+    return r;
+}
+// Copy of the vector at element `at` of a tensor of `count`, and the vector itself once it has arrived.
+template <class T, int V, bool S>
+__device__ __forceinline__ void copy_vector(Pack<T, V>* to, const T* base, uint64_t at, uint64_t count) {
+    if constexpr (!S) {
+        copy_async<T, V>(to, base, at, count);
+    } else {
+        const uint64_t first = at & ~(uint64_t)(V - 1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint64_t e = first + k * V;
+            const uint32_t have = e >= count ? 0u : count - e < V ? (uint32_t)(count - e) * (uint32_t)sizeof(T) : 16u;
+            if (have)  // what lies behind the tensor is not read
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to + k * blockDim.x)),
+                             "l"(base + e), "r"(have) : "memory");
+        }
+    }
+}
+template <class T, int V, bool S>
+__device__ __forceinline__ Pack<T, V> read_vector(const Pack<T, V>* from, uint64_t at) {
+    if constexpr (S) return across<T, V>(from[0], from[blockDim.x], (uint32_t)at & (V - 1));
+    else return read<T, V>(from, at);
+}
+// Elements from `valid` on become 0.
+template <int V>
+__device__ __forceinline__ void cut(float (&f)[V], uint32_t valid) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = j < valid ? f[j] : 0.0f;
+}
+template <class T, int V>
+__device__ __forceinline__ void store_elements(T* out, uint64_t at, const Pack<T, V>& o, uint32_t from, uint32_t to) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j >= from && j < to) {
+            ((uint16_t*)out)[at + j] = (uint16_t)(j & 1 ? o.w[j / 2] >> 16 : o.w[j / 2]);
+        }
+}
+// Stores the first `valid` elements of a vector for every thread of a warp with ok; neighbouring threads have
+// neighbouring vectors. All threads of the warp call it.
+template <class T, int V>
+__device__ __forceinline__ void store_shifted(T* out, uint64_t at, const Pack<T, V>& o, bool ok, uint32_t valid) {
+    const uint32_t lane = threadIdx.x & 31, shift = (uint32_t)at & (V - 1), own = V - shift;  // own: of the vector it starts in
+    Pack<T, V> before;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) before.w[k] = __shfl_up_sync(~0u, o.w[k], 1);
+    const uint32_t oks = __ballot_sync(~0u, ok);
+    if (!ok) return;
+    const bool left = lane > 0 && (oks >> (lane - 1) & 1u), right = lane < 31 && (oks >> (lane + 1) & 1u);
+    if (shift == 0) {
+        if (valid == V) o.store(out + at);
+        else store_elements(out, at, o, 0, valid);
+        return;
+    }
+    if (left && valid >= own) {
+        across<T, V>(before, o, own).store(out + (at - shift));
+    } else {
+        if (left) store_elements(out, at - V, before, own, V);
+        store_elements(out, at, o, 0, valid < own ? valid : own);
+    }
+    if (!right) store_elements(out, at, o, own, valid);  // nobody to pass them to
+}
+
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void copy_wait() {

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
     const GroupWalk walk = group_walk<V, L>(a, t, tid);
     float acc_a[V] = {}, acc_b[V] = {};
     for (uint32_t n = blockIdx.x / p.tiles; n < a.n; n += gridDim.x / p.tiles) {
-        const uint64_t at = (n * p.vecs + row * p.rv + col) * V;
+        const uint64_t at = n * p.elems + (uint64_t)(row * p.rv + col) * V;
         Pack<T, V> rx[kBatchBwd], rv[kBatchBwd];
 #pragma unroll
         for (int i = 0; i < kBatchBwd; ++i)
@@ -230,16 +230,16 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
 // 637 MB cross DRAM, 5.6 TB/s, 86 % of the measured copy rate; read and written once it would be 61 us. 8 x 64 x 64 x
 // 256 takes 25 us against 7.7: 9 us for the first pass (34 MB, with two special-function uses and about 90 FP32
 // operations a vector lane), 5 for sums, barrier and join, 6 for the second pass, 1 to 2 for the channels.
-template <class T, int V, int L, int ACT, int DROP>
+template <class T, int V, int L, int ACT, int DROP, bool S>
 __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
-    constexpr int P = kParts<V, L>, R = kRowsBwd, F = kAheadBwd;
+    constexpr int P = kParts<V, L>, R = rows_of_batch(true, S), F = batches_ahead(true, S), E = S ? 2 : 1;
     const uint32_t tid = threadIdx.x, threads = blockDim.x, tile_c = p.tiles == 1 ? a.c : p.cols * V;
     float2* sum = (float2*)smem;            // [gl]
     float2* warp_sum = sum + p.gl;          // [warps]
     float2* chan = warp_sum + kThreads / 32;  // [tile_c]
     float* part = (float*)(((uintptr_t)(chan + tile_c) + 15) & ~(uintptr_t)15);  // [2] places<V>
-    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + 2 * places<V>(threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][x, v][threads]
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + 2 * places<V>(threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][x, v][E][threads]
     const Run run = run_of(a, p);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
@@ -249,19 +249,19 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
     float2* slots = (float2*)a.ws;                                                   // [(block + unit) gl + group]
     float2* chans = slots + (uint64_t)(gridDim.x * gridDim.y + p.tiles * (uint32_t)a.n) * p.gl;  // [(block + tile) tile_c + channel - c0]
     const bool wanted = a.v_weight || a.v_bias;
-    const uint64_t count = a.n * p.vecs * V;  // elements
+    const uint64_t count = a.n * p.elems;
 
     Walk<V, R> ahead;
     ahead.u = run.first;
     ahead.unit(a, p, run, false);
     uint32_t to_slot = 0, slot = 0;
     const auto copy = [&]() {
-        Pack<T, V>* to = ring + to_slot * 2 * R * threads;
+        Pack<T, V>* to = ring + to_slot * 2 * R * E * threads;
 #pragma unroll
         for (int j = 0; j < R; ++j)
             if (ahead.i + j < ahead.valid) {
-                copy_async<T, V>(to + 2 * j * threads, (const T*)a.x, ahead.at + j * step, count);
-                copy_async<T, V>(to + (2 * j + 1) * threads, (const T*)a.v, ahead.at + j * step, count);
+                copy_vector<T, V, S>(to + 2 * j * E * threads, (const T*)a.x, ahead.at + j * step, count);
+                copy_vector<T, V, S>(to + (2 * j + 1) * E * threads, (const T*)a.v, ahead.at + j * step, count);
             }
     };
 #pragma unroll 1
@@ -291,33 +291,41 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
 #pragma unroll
         for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.0f;
         uint64_t at = g.at;
-        const auto take = [&](const Pack<T, V>* px, Pack<T, V>* in, uint64_t where) {
+        const auto take = [&](const Pack<T, V>* px, Pack<T, V>* in, uint64_t where, bool cut_short) {
             float fx[V], fv[V];
-            Pack<T, V> pv = read(in, where);
-            read(px, where).get(fx);
+            Pack<T, V> pv = read_vector<T, V, S>(in, where);
+            read_vector<T, V, S>(px, where).get(fx);
             if (drops<DROP>(a)) {
-                drop_packed(a.drop, dstep, where, pv);
-                if (batch >= resident) {  // the second pass need not draw again
+                drop_packed<S>(a.drop, dstep, where, pv);
+                if (!S && batch >= resident) {  // the second pass need not draw again
                     if (V * sizeof(T) == 2) pv.w[0] |= pv.w[0] << 16;
                     *in = pv;
                 }
             }
             pv.get(fv);
+            if (S && cut_short) {  // two lanes share a reciprocal, and so its rounding
+                cut<V>(fx, p.tail);
+                cut<V>(fv, p.tail);
+            }
             if (drops<DROP>(a)) mul_v<V>(fv, fv, scale);
             lanes.grads(act_of<ACT>(a), fx, fv);
+            if (S && cut_short) {
+                cut<V>(fx, p.tail);
+                cut<V>(fv, p.tail);
+            }
             accumulate<V, V>(sa, fv);
             accumulate<V, V>(sb, fv, fx);
         };
         for (uint32_t i0 = 0; i0 < g.iters; i0 += R, ++batch) {
             copy_wait<F - 1>();
-            Pack<T, V>* have = ring + slot * 2 * R * threads;
+            Pack<T, V>* have = ring + slot * 2 * R * E * threads;
             if (i0 + R <= g.cnt) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) take(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
+                for (int j = 0; j < R; ++j) take(have + 2 * j * E * threads, have + (2 * j + 1) * E * threads, at + j * step, i0 + j + 1 == g.tail);
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) take(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
+                    if (i0 + j < g.cnt) take(have + 2 * j * E * threads, have + (2 * j + 1) * E * threads, at + j * step, i0 + j + 1 == g.tail);
             }
             at += R * step;
             slot = slot + 1 == p.ring ? 0 : slot + 1;
@@ -382,30 +390,46 @@ __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, co
         });
         if (g.cnt) gg.take(a, p, t, g.c, sum, m, lanes);
         uint64_t at = g.at + (g.iters - 1) / R * R * step;
-        const auto give = [&](const Pack<T, V>* px, const Pack<T, V>* in, uint64_t where) {
+        const auto give = [&](const Pack<T, V>* px, const Pack<T, V>* in, uint64_t where, bool cut_short) {
             float fx[V], fv[V];
-            Pack<T, V> pv = read(in, where);
-            read(px, where).get(fx);
-            if (drops<DROP>(a) && batch < resident) drop_packed(a.drop, dstep, where, pv);
+            Pack<T, V> pv = read_vector<T, V, S>(in, where);
+            read_vector<T, V, S>(px, where).get(fx);
+            if (drops<DROP>(a) && (S || batch < resident)) drop_packed<S>(a.drop, dstep, where, pv);
             pv.get(fv);
+            if (S && cut_short) {
+                cut<V>(fx, p.tail);
+                cut<V>(fv, p.tail);
+            }
             if (drops<DROP>(a)) mul_v<V>(fv, fv, scale);
             lanes.grads(act_of<ACT>(a), fx, fv);
             gg.apply(lanes, fx, fv);
             Pack<T, V> o;
             o.set(fx);
-            o.store((T*)a.out + where);
+            return o;
         };
         for (uint32_t i0 = (g.iters - 1) / R * R;; i0 -= R) {
             --batch;
             copy_wait<F - 1>();
-            const Pack<T, V>* have = ring + slot * 2 * R * threads;
-            if (i0 + R <= g.cnt) {
+            const Pack<T, V>* have = ring + slot * 2 * R * E * threads;
+            if constexpr (S) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) give(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
+                for (int j = 0; j < R; ++j) {  // all threads: neighbours exchange what they store
+                    const uint64_t where = at + j * step;
+                    const bool ok = i0 + j < g.cnt;
+                    Pack<T, V> o{};
+                    const bool cut_short = i0 + j + 1 == g.tail;
+                    if (ok) o = give(have + 2 * j * E * threads, have + (2 * j + 1) * E * threads, where, cut_short);
+                    store_shifted<T, V>((T*)a.out, where, o, ok, cut_short ? p.tail : V);
+                }
+            } else if (i0 + R <= g.cnt) {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    give(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step, false).store((T*)a.out + at + j * step);
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) give(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step);
+                    if (i0 + j < g.cnt)
+                        give(have + 2 * j * threads, have + (2 * j + 1) * threads, at + j * step, false).store((T*)a.out + at + j * step);
             }
             at -= R * step;
             slot = slot == 0 ? p.ring - 1 : slot - 1;

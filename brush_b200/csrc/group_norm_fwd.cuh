@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads, 2) small_fwd_kernel(const Plan p, co
     const bool active = row < p.k;
     const uint32_t rows = p.rows - (col >= p.last);  // of this column
     const uint32_t step = p.k * p.rv * V;
-    const uint64_t at = (n * p.vecs + row * p.rv + col) * V;
+    const uint64_t at = n * p.elems + (uint64_t)(row * p.rv + col) * V;
     const T* x = (const T*)a.x + at;
     Pack<T, V> raw[kBatch];
     uint32_t cnt = 0;
@@ -122,10 +122,10 @@ __global__ void __launch_bounds__(kThreads, 2) small_fwd_kernel(const Plan p, co
 }
 
 // Large samples: one cooperative launch. Every thread copies its vectors of the block's coming batches of rows into
-// its own places of a ring in shared memory, kAhead batches ahead. First pass: mean and sum of squared deviations of
+// its own places of a ring in shared memory, some batches ahead. First pass: mean and sum of squared deviations of
 // each group in each segment, to the workspace. Deviations are taken from a pivot, the group's mean over the block's
-// first batch, so that no large mean cancels (what the pivot is off by enters the sum of squares at most rows / kRows
-// times over). Grid barrier. Second pass, last row first: the segments' statistics are joined, and the rows are
+// first batch, so that no large mean cancels (what the pivot is off by enters the sum of squares at most a quarter of
+// the block's rows times over). Grid barrier. Second pass, last row first: the segments' statistics are joined, and the rows are
 // normalised out of the ring, which still holds the last ones; the others come again.
 // A full frame of 64 bf16 channels (265 MB, larger than L2) takes 139 us: 27 MB stay in the rings, so 765 MB cross
 // DRAM, 5.5 TB/s, 84 % of the measured copy rate; read once and written once it would be 81 us. Keeping more in L2
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2) small_fwd_kernel(const Plan p, co
 // nothing. 8 x 64 x 64 x 256 (17 MB, all of it stays) takes 15.5 us against 5.1: 5 us until the last row has arrived,
 // 1 for the sums, 1.5 each for the barrier and the join, 4 for the second pass, which the special-function unit
 // bounds (three uses for two elements, four lanes a cycle and scheduler), the rest launch and prologue.
-template <class T, int V, int L, int ACT, int DROP>
+template <class T, int V, int L, int ACT, int DROP, bool S>
 __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
     float2* sum = (float2*)smem;                       // [gl]
@@ -141,12 +141,12 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
     float* pivot = (float*)(warp_sum + kThreads / 32);  // [gl]: later the mean of the block's segment
     float* part = (float*)(((uintptr_t)(pivot + p.gl) + 15) & ~(uintptr_t)15);  // [2] places<L>
     const uint32_t tid = threadIdx.x, threads = blockDim.x;
-    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + 2 * places<L>(threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][threads]
-    constexpr int P = kParts<V, L>, R = kRows, F = kAhead;
+    Pack<T, V>* ring = (Pack<T, V>*)(((uintptr_t)(part + 2 * places<L>(threads)) + 15) & ~(uintptr_t)15) + tid;  // [ring][R][E][threads]
+    constexpr int P = kParts<V, L>, R = rows_of_batch(false, S), F = batches_ahead(false, S), E = S ? 2 : 1;
     const Run run = run_of(a, p);
     const uint64_t step = (uint64_t)run.stride * p.rv * V;
     const uint32_t all = batches_of<R>(p, run);
-    const uint64_t count = a.n * p.vecs * V;  // elements
+    const uint64_t count = a.n * p.elems;
     float2* slots = (float2*)a.ws;  // [(block + unit) gl + group]: mean, squared deviations
 
     Walk<V, R> ahead;
@@ -154,14 +154,14 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
     ahead.unit(a, p, run, false);
     uint32_t to_slot = 0, slot = 0;  // ring places of the batch to copy and of the batch at work
     const auto copy = [&]() {
-        Pack<T, V>* to = ring + to_slot * R * threads;
+        Pack<T, V>* to = ring + to_slot * R * E * threads;
         if (ahead.i + R <= ahead.valid) {
 #pragma unroll
-            for (int j = 0; j < R; ++j) copy_async<T, V>(to + j * threads, (const T*)a.x, ahead.at + j * step, count);
+            for (int j = 0; j < R; ++j) copy_vector<T, V, S>(to + j * E * threads, (const T*)a.x, ahead.at + j * step, count);
         } else {
 #pragma unroll
             for (int j = 0; j < R; ++j)
-                if (ahead.i + j < ahead.valid) copy_async<T, V>(to + j * threads, (const T*)a.x, ahead.at + j * step, count);
+                if (ahead.i + j < ahead.valid) copy_vector<T, V, S>(to + j * E * threads, (const T*)a.x, ahead.at + j * step, count);
         }
     };
 #pragma unroll 1
@@ -183,12 +183,13 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
         float off[L], acc[P] = {}, sq[P] = {}, all_acc[P] = {}, all_sq[P] = {}, val[L], val2[L];
         copy_wait<F - 1>();
         {
-            const Pack<T, V>* at = ring + slot * R * threads;
+            const Pack<T, V>* at = ring + slot * R * E * threads;
 #pragma unroll
             for (int j = 0; j < R; ++j)
                 if (j < g.cnt) {
                     float f[V];
-                    read(at + j * threads, g.at + j * step).get(f);
+                    read_vector<T, V, S>(at + j * E * threads, g.at + j * step).get(f);
+                    if (S && j + 1 == g.tail) cut<V>(f, p.tail);
                     accumulate<V, L>(acc, f);
                 }
             per_item<V, L>(acc, val);
@@ -208,23 +209,24 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
 #pragma unroll
             for (int j = 0; j < P; ++j) acc[j] = 0.0f;
         }
-        const auto take = [&](const Pack<T, V>& v) {
+        const auto take = [&](const Pack<T, V>& v, uint32_t i) {
             float f[V];
             v.get(f);
             add_v<V>(f, f, off);
+            if (S && i + 1 == g.tail) cut<V>(f, p.tail);
             accumulate<V, L>(acc, f);
             accumulate<V, L>(sq, f, f);
         };
         for (uint32_t i0 = 0; i0 < g.iters; i0 += R, ++batch) {
             copy_wait<F - 1>();
-            const Pack<T, V>* at = ring + slot * R * threads;
+            const Pack<T, V>* at = ring + slot * R * E * threads;
             if (i0 + R <= g.cnt) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) take(read(at + j * threads, g.at + (i0 + j) * step));
+                for (int j = 0; j < R; ++j) take(read_vector<T, V, S>(at + j * E * threads, g.at + (i0 + j) * step), i0 + j);
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) take(read(at + j * threads, g.at + (i0 + j) * step));
+                    if (i0 + j < g.cnt) take(read_vector<T, V, S>(at + j * E * threads, g.at + (i0 + j) * step), i0 + j);
             }
             slot = slot + 1 == p.ring ? 0 : slot + 1;
             if (batch + F < all) {
@@ -302,26 +304,39 @@ __global__ void __launch_bounds__(kThreads, 1) large_fwd_kernel(const Plan p, co
         __syncthreads();
         if (g.cnt) lanes.fold(a, p, t, g.c, sum);
         uint64_t at = g.at + (g.iters - 1) / R * R * step;
-        const auto give = [&](const Pack<T, V>& v, uint64_t where) {
+        const auto give = [&](const Pack<T, V>& v, uint64_t where, bool cut_short) {
             float f[V];
             v.get(f);
+            if (S && cut_short) cut<V>(f, p.tail);  // two lanes share a reciprocal, and so its rounding
             lanes.apply(act_of<ACT>(a), f);
-            if (drops<DROP>(a)) drop_vector<V>(a.drop, dstep, where, f);
+            if (drops<DROP>(a)) drop_vector<V, S>(a.drop, dstep, where, f);
             Pack<T, V> o;
             o.set(f);
-            o.store((T*)a.out + where);
+            return o;
         };
         for (uint32_t i0 = (g.iters - 1) / R * R;; i0 -= R) {
             --batch;
             copy_wait<F - 1>();
-            const Pack<T, V>* have = ring + slot * R * threads;
-            if (i0 + R <= g.cnt) {
+            const Pack<T, V>* have = ring + slot * R * E * threads;
+            if constexpr (S) {
 #pragma unroll
-                for (int j = 0; j < R; ++j) give(read(have + j * threads, at + j * step), at + j * step);
+                for (int j = 0; j < R; ++j) {  // all threads: neighbours exchange what they store
+                    const uint64_t where = at + j * step;
+                    const bool ok = i0 + j < g.cnt;
+                    Pack<T, V> o{};
+                    const bool cut_short = i0 + j + 1 == g.tail;
+                    if (ok) o = give(read_vector<T, V, S>(have + j * E * threads, where), where, cut_short);
+                    store_shifted<T, V>((T*)a.out, where, o, ok, cut_short ? p.tail : V);
+                }
+            } else if (i0 + R <= g.cnt) {
+#pragma unroll
+                for (int j = 0; j < R; ++j)
+                    give(read_vector<T, V, S>(have + j * threads, at + j * step), at + j * step, false).store((T*)a.out + at + j * step);
             } else {
 #pragma unroll
                 for (int j = 0; j < R; ++j)
-                    if (i0 + j < g.cnt) give(read(have + j * threads, at + j * step), at + j * step);
+                    if (i0 + j < g.cnt)
+                        give(read_vector<T, V, S>(have + j * threads, at + j * step), at + j * step, false).store((T*)a.out + at + j * step);
             }
             at -= R * step;
             slot = slot == 0 ? p.ring - 1 : slot - 1;

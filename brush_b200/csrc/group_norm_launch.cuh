@@ -42,20 +42,20 @@ cudaError_t cooperative(K kernel, const Args& a, const Plan& p, dim3 blocks, uin
     return cudaLaunchKernelEx(&cfg, kernel, p, a);
 }
 
-template <class T, int V, int L, int ACT, int DROP, bool BWD>
+template <class T, int V, int L, int ACT, int DROP, bool BWD, bool S = false>
 cudaError_t launch_one(const Call& c) {
     const Args& a = *c.a;
     Plan& p = *c.p;
     const int sms = sm_count(c.device);
     const uint32_t sums = 8 * (p.gl + kThreads / 32);  // sum, warp_sum
-    if constexpr (!BWD) if (p.small) {
+    if constexpr (!BWD && !S) if (p.small) {
         static std::atomic<uint64_t> done{0};
         auto k = small_fwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
         k<<<p.blocks, p.threads, sums + 16 + 4 * (p.gl + places<L>(p.threads)), c.stream>>>(p, a);
         return cudaSuccess;
     }
-    if constexpr (BWD) if (p.small) {
+    if constexpr (BWD && !S) if (p.small) {
         static std::atomic<uint64_t> done{0};
         auto k = small_bwd_kernel<T, V, L, ACT, DROP>;
         if (cudaError_t e = prepare(k, done, c.device)) return e;
@@ -77,7 +77,7 @@ cudaError_t launch_one(const Call& c) {
     }
     const uint32_t tile_c = p.tiles == 1 ? a.c : p.cols * V;
     const uint32_t head = 32 + sums + (BWD ? 8 * (tile_c + places<V>(p.threads)) : 4 * p.gl + 8 * places<L>(p.threads));
-    const uint32_t row = p.threads * (uint32_t)sizeof(Pack<T, V>) * (BWD ? 2 : 1);  // a single 16-bit element takes a word
+    const uint32_t row = p.threads * (uint32_t)sizeof(Pack<T, V>) * (BWD ? 2 : 1) * (S ? 2 : 1);  // a single 16-bit element takes a word
     // Where units are few, each has blocks of its own, so that no block sums and joins twice; where that would
     // leave more than a tenth of the SMs idle, runs cross units.
     const uint32_t units = (uint32_t)a.n * p.tiles, total = p.rows * units;
@@ -93,7 +93,8 @@ cudaError_t launch_one(const Call& c) {
         p.per_block = (total + blocks - 1) / blocks;
         blocks = (total + p.per_block - 1) / p.per_block;
     }
-    const uint32_t rows = BWD ? kRowsBwd : kRows, batch = rows * row;
+    constexpr uint32_t rows = rows_of_batch(BWD, S);
+    const uint32_t batch = rows * row;
     // the longest run's batches: its rows, and a cut batch at each end of a unit
     const uint32_t longest = p.per_block / rows + 1 + (p.per_unit ? 0 : p.per_block / p.rows + 1);
     p.ring = (kSharedMost - 16 - head) / batch;
@@ -102,8 +103,8 @@ cudaError_t launch_one(const Call& c) {
     const dim3 grid = p.per_unit ? dim3(p.per_unit, units) : dim3(blocks);
     static std::atomic<uint64_t> done{0};
     const auto k = [] {
-        if constexpr (BWD) return large_bwd_kernel<T, V, L, ACT, DROP>;
-        else return large_fwd_kernel<T, V, L, ACT, DROP>;
+        if constexpr (BWD) return large_bwd_kernel<T, V, L, ACT, DROP, S>;
+        else return large_fwd_kernel<T, V, L, ACT, DROP, S>;
     }();
     if (cudaError_t e = prepare(k, done, c.device)) return e;
     return cooperative(k, a, p, grid, bytes, c.stream);
@@ -124,6 +125,7 @@ cudaError_t by_act(const Call& c) {
 template <class T, bool BWD>
 cudaError_t launch(const Call& c) {
     constexpr int M = 16 / (int)sizeof(T);
+    if constexpr (M == 8) if (c.p->shifted) return launch_one<T, M, M, kAny, kAny, BWD, true>(c);
     if (c.p->v == M) {
         if (c.items == 1) return by_act<T, M, 1, BWD>(c);
         if (c.items == 2) return by_act<T, M, 2, BWD>(c);

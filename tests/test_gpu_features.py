@@ -358,6 +358,62 @@ def test_group_norm_gradient_against_differences(cuda):
     assert abs(got - num) <= bound + 1e-6 * scale
 
 
+# Samples of an odd number of elements: large ones, read across vectors in 16 bits (one and many of them, a block's rows
+# crossing them, a channel a group and one group, last vectors of every odd length), and smaller and even ones.
+SHIFTED = [(1, (80_001,), 37, 37), (2, (100_001,), 37, 1), (3, (7777,), 185, 5), (3, (2001,), 511, 7), (1, (1_000_001,), 3, 3),
+           (200, (501,), 37, 1), (61, (4801,), 9, 3), (9, (60_007,), 5, 1), (7, (18_003,), 21, 7), (4, (20_001,), 3, 3),
+           (3, (1235, 21), 12, 4), (2, (9001,), 14, 7)]
+
+
+@pytest.mark.parametrize("shape", SHIFTED, ids=lambda s: f"{s[0]}x{'x'.join(map(str, s[1]))}x{s[2]}g{s[3]}")
+@pytest.mark.parametrize("dtype,act,p", [(torch.float32, "silu", 0.2), (torch.bfloat16, "gelu_tanh", 0.0),
+                                         (torch.bfloat16, "silu", 0.3), (torch.float16, "none", 0.5)],
+                         ids=lambda v: str(v).replace("torch.", ""))
+def test_group_norm_samples_off_a_vector(cuda, shape, dtype, act, p):
+    import brush_b200 as bsx
+
+    x, w, b, v = _inputs(shape, dtype, "f32", 70)
+    g = shape[3]
+    drop = bsx.DropoutConfig(p=p, seed=31, step=2) if p else None
+    cfg = bsx.GroupNormConfig(groups=g, activation=act, dropout=drop)
+    r = ref.GroupNorm(x, w, b, g, act=act, drop=(ref.mask(x.numel(), p, 31, 2), p) if p else None)
+    d = [t.cuda() for t in (x, w, b, v)]
+    stats = [t.float().cuda() for t in (r.mean, r.rstd)]
+    once = [bsx.group_norm_forward(*d[:3], cfg), bsx.group_norm_backward(d[3], *d[:3], *stats, cfg)]
+    for got, want in zip(once[0], r.forward()):
+        ref.close(got, want)
+    for got, want in zip(once[1], r.backward(v)):
+        ref.close(got, want)
+    again = [bsx.group_norm_forward(*d[:3], cfg), bsx.group_norm_backward(d[3], *d[:3], *stats, cfg)]
+    for a, c in zip(once, again):
+        assert all(torch.equal(s, t) for s, t in zip(a, c))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [0, 1, 2])
+def test_group_norm_neighbours_of_a_bad_sample(cuda, dtype, bad):
+    # A vector across two samples holds values of both: a sample of NaN leaves the others as they are, bit for bit.
+    import brush_b200 as bsx
+
+    x, w, b, v = (t.cuda() for t in _inputs((3, (25_001,), 37, 37), dtype, "f32", 75))
+    cfg = bsx.GroupNormConfig(groups=37, activation="silu", dropout=bsx.DropoutConfig(p=0.25, seed=4, step=1))
+    out, mean, rstd = bsx.group_norm_forward(x, w, b, cfg)
+    vx = bsx.group_norm_backward(v, x, w, b, mean, rstd, cfg)[0]
+    x2, v2 = x.clone(), v.clone()
+    x2[bad] = float("nan")
+    v2[bad] = float("nan")
+    out2, mean2, rstd2 = bsx.group_norm_forward(x2, w, b, cfg)
+    vx2 = bsx.group_norm_backward(v2, x2, w, b, mean2, rstd2, cfg)[0]
+    for k in range(3):
+        if k == bad:
+            assert mean2[k].isnan().all() and rstd2[k].isnan().all()
+            kept = ref.mask(x.numel(), 0.25, 4, 1).view(3, 25_001, 37)[k]
+            assert torch.equal(out2[k].isnan().cpu(), kept) and (out2[k].cpu()[~kept] == 0).all()
+        else:
+            for one, two in ((out, out2), (mean, mean2), (rstd, rstd2), (vx, vx2)):
+                assert torch.equal(one[k], two[k])
+
+
 @pytest.mark.parametrize("shape", [(3, (20, 20), 64, 8), (2, (300, 200), 48, 8), (2, (31, 17), 37, 37)])
 def test_group_norm_repeats_bit_for_bit(cuda, shape):
     import brush_b200 as bsx
