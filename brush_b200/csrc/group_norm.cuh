@@ -203,9 +203,13 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // (gelu in its tanh form, because (1 + tanh(t)) / 2 = s(2 t)). With e = 2^(-w log2 e) it is
 // s = 1 / (1 + e). The special-function unit takes eight cycles for an exponential or reciprocal
 // of a warp and would bound a pass over 16-bit data, so two reciprocals are one of the product:
-// 1 / a = b / (a b). Exponents are held below 60 so that the product stays finite: s is right to
-// a few units in the last place above 2^-60, and 2^-60 below.
+// 1 / a = b / (a b). Exponents are held at 63 so that the product stays finite. What they leave,
+// 2^-63, must not be multiplied by a far z, nor by the slope's terms, which grow with it: 2^-62 is
+// taken off every s and the result clamped to [0, 1], both in the multiplication that forms it. s is
+// off by a few units in the last place, by |w| of them (the rounding of w log2 e) and by 2^-62, and
+// is 0 from w = -43.7 down.
 constexpr float kLog2e = 1.4426950408889634f, kGelu1 = 1.5957691216057308f, kGelu3 = 0.044715f;
+constexpr float kMostExponent = 63.0f, kLeft = 2.168404344971009e-19f;  // 2^-62
 template <int V>
 __device__ __forceinline__ void gates(int act, const float (&z)[V], float (&s)[V], float (&e)[V]) {
     constexpr float one[1] = {1.0f};
@@ -219,16 +223,16 @@ __device__ __forceinline__ void gates(int act, const float (&z)[V], float (&s)[V
         mul_v<V>(e, e, z);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) e[j] = exp2_fast(fminf(e[j], 60.0f));
+    for (int j = 0; j < V; ++j) e[j] = exp2_fast(fminf(e[j], kMostExponent));
     add_v<V>(s, e, one);
     if constexpr (V == 1) {
-        s[0] = rcp_fast(s[0]);
+        s[0] = __saturatef(rcp_fast(s[0]) - kLeft);
     } else {
 #pragma unroll
         for (int j = 0; j < V; j += 2) {
             const float r = rcp_fast(s[j] * s[j + 1]), other = s[j];
-            s[j] = s[j + 1] * r;
-            s[j + 1] = other * r;
+            s[j] = __saturatef(__fmaf_rn(s[j + 1], r, -kLeft));
+            s[j + 1] = __saturatef(__fmaf_rn(other, r, -kLeft));
         }
     }
 }
@@ -239,26 +243,32 @@ __device__ __forceinline__ void activate(int act, float (&z)[V]) {
     gates<V>(act, z, s, e);
     mul_v<V>(z, z, s);
 }
-// v act'(z): act'(z) = s + s (1 - s) z w'(z) = s (1 + e s z w'(z)): 1 - s = e s without a difference. NaN goes
-// through z.
+// v act'(z): act'(z) = s + s (1 - s) z w'(z) = s (1 + c z w'(z)) with c = 1 - s = e s without a difference. NaN goes
+// through z. c z is formed first: it is 0 on both sides far from 0, where w' grows without bound but, z being at most
+// about kMostBias, stays finite.
 template <int V>
 __device__ __forceinline__ void back_activate(int act, float (&v)[V], float (&z)[V]) {
     if (act == BSX_ACT_NONE) return;
     constexpr float one[1] = {1.0f};
-    float s[V], e[V];
-    gates<V>(act, z, s, e);
-    mul_v<V>(e, e, s);
+    float s[V], c[V];
+    gates<V>(act, z, s, c);
+    mul_v<V>(c, c, s);
+    mul_v<V>(c, c, z);
     if (act == BSX_ACT_GELU_TANH) {
         constexpr float k1[1] = {kGelu1}, k3[1] = {3.0f * kGelu1 * kGelu3};
-        float t[V];
-        mul_v<V>(t, z, z);
-        fma_v<V>(t, t, k3, k1);
-        mul_v<V>(z, z, t);
+        mul_v<V>(z, z, z);
+        fma_v<V>(z, z, k3, k1);
+        fma_v<V>(z, z, c, one);
+    } else {
+        add_v<V>(z, c, one);
     }
-    fma_v<V>(z, e, z, one);
     mul_v<V>(z, z, s);
     mul_v<V>(v, v, z);
 }
+// The slope's z of gelu is formed from biases within this: farther ones (channels switched off by the type's lowest value)
+// have the same slope, 0 or 1, and a w' that would overflow. NaN stays.
+constexpr float kMostBias = 4611686018427387904.0f;  // 2^62
+__device__ __forceinline__ float near_bias(float b) { return b > kMostBias ? kMostBias : b < -kMostBias ? -kMostBias : b; }
 
 // Bit j: element j of a vector at flat element `at` is kept; a vector may lie across two blocks of draws.
 template <int V>

@@ -17,6 +17,10 @@ struct GradLanes {
     __device__ __forceinline__ void load(const Args& a, uint32_t c) {
         params<T, V>(a, a.weight, c, 1.0f, w);
         params<T, V>(a, a.bias, c, 0.0f, b);
+        if (a.act == BSX_ACT_GELU_TANH) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) b[j] = near_bias(b[j]);
+        }
     }
     __device__ __forceinline__ void stats(const Args& a, const Plan& p, uint64_t n, uint32_t c) {
 #pragma unroll
