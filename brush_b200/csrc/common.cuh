@@ -146,7 +146,9 @@ struct bsx_fwd_state {
 struct bsx_ctx {
     int device = 0;
     cudaStream_t stream = nullptr;
-    std::string last_error;
+    uint64_t id = 0;         // of this process's contexts, from 1
+    mutable std::mutex error_mutex;
+    std::string last_error;  // under error_mutex: of whichever thread failed last
     uint64_t launches = 0;
     int* d_err = nullptr;            // device error word
     uint32_t* h_pinned = nullptr;    // pinned readback slots

@@ -1,5 +1,6 @@
 // ctx.cu - context lifetime, error reporting, workspace growth and the
 // host-side camera -> uniforms computation.
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -8,8 +9,22 @@
 
 namespace bsx {
 
+namespace {
+// A thread's last failing call, and what bsx_last_error handed to it: texts that no other thread changes.
+struct ThreadError {
+    uint64_t ctx = 0;
+    std::string text, other;
+};
+thread_local ThreadError t_error;
+}  // namespace
+
 bsx_status fail(bsx_ctx* ctx, bsx_status s, const std::string& msg) {
-    if (ctx) ctx->last_error = msg;
+    if (ctx) {
+        t_error.ctx = ctx->id;
+        t_error.text = msg;
+        std::lock_guard<std::mutex> lock(ctx->error_mutex);
+        ctx->last_error = msg;
+    }
     return s;
 }
 
@@ -121,6 +136,8 @@ bsx_status bsx_create(int device, bsx_ctx** out) {
     *out = nullptr;
     bsx_ctx* ctx = new (std::nothrow) bsx_ctx();
     if (!ctx) return BSX_ERR_INVALID_ARG;
+    static std::atomic<uint64_t> contexts{0};
+    ctx->id = ++contexts;
     ctx->device = device;
     cudaError_t e = cudaSetDevice(device);
     if (e == cudaSuccess) e = cudaMalloc(&ctx->d_err, 256);
@@ -204,7 +221,17 @@ bsx_status bsx_sync(bsx_ctx* ctx) {
     return check_device_error(ctx);
 }
 
-const char* bsx_last_error(const bsx_ctx* ctx) { return ctx ? ctx->last_error.c_str() : "null context"; }
+const char* bsx_last_error(const bsx_ctx* ctx) {
+    if (!ctx) return "null context";
+    if (t_error.ctx == ctx->id) return t_error.text.c_str();
+    try {
+        std::lock_guard<std::mutex> lock(ctx->error_mutex);
+        t_error.other = ctx->last_error;
+    } catch (...) {
+        return "";
+    }
+    return t_error.other.c_str();
+}
 
 uint64_t bsx_launch_count(const bsx_ctx* ctx) { return ctx ? ctx->launches : 0; }
 

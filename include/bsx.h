@@ -175,6 +175,9 @@ BSX_API bsx_status bsx_set_stream(bsx_ctx* ctx, void* cuda_stream);
  * bsx_render_out pointer. */
 BSX_API bsx_status bsx_trim(bsx_ctx* ctx);
 BSX_API bsx_status bsx_sync(bsx_ctx* ctx);
+/* Text of the calling thread's last failing call if that was on this context, else of the
+ * context's last failing call on any thread. It stays valid until the thread's next failing
+ * call or next bsx_last_error. */
 BSX_API const char* bsx_last_error(const bsx_ctx* ctx);
 BSX_API const char* bsx_status_string(bsx_status s);
 BSX_API int bsx_abi_version(void);
