@@ -4,9 +4,11 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <string>
+#include <thread>
 #include <vector>
 
 #include "../../include/bsx.h"
@@ -149,7 +151,7 @@ struct bsx_ctx {
     uint64_t id = 0;         // of this process's contexts, from 1
     mutable std::mutex error_mutex;
     std::string last_error;  // under error_mutex: of whichever thread failed last
-    uint64_t launches = 0;
+    std::atomic<uint64_t> launches{0};
     int* d_err = nullptr;            // device error word
     uint32_t* h_pinned = nullptr;    // pinned readback slots
     // workspace
@@ -161,18 +163,18 @@ struct bsx_ctx {
         // percentile bounds of the means (bounds.cu)
         bounds_tmp;
     bsx_fwd_state fwd;
-    // the feature operators (dropout.cu, group_norm.cu) may be called from several threads at once
-    std::mutex op_mutex;
-    // optional per-launch timing (bsx_profile_*)
-    int profiling = 0;
-    cudaEvent_t prof_start = nullptr;
+    // optional per-launch timing (bsx_profile_*); the feature operators (dropout.cu, group_norm.cu) may be
+    // called from several threads at once, beside the calls of the context's own stream
+    std::atomic<int> profiling{0};
     struct ProfRec {
         const char* name;
         cudaEvent_t a, b;
     };
+    mutable std::mutex prof_mutex;  // of what follows
+    std::map<std::thread::id, cudaEvent_t> prof_start;  // of the launch that a thread is at
     std::vector<ProfRec> prof_pending;
     std::vector<cudaEvent_t> prof_pool;
-    std::vector<std::string> prof_names;
+    std::vector<const char*> prof_names;
     std::vector<double> prof_ms;
     std::vector<uint64_t> prof_count;
 };
@@ -184,7 +186,7 @@ bsx_status check_cuda(bsx_ctx* ctx, cudaError_t e, const char* what);
 bsx_status ensure(bsx_ctx* ctx, DevBuf& b, size_t bytes);
 // Stream-ordered release of a workspace buffer.
 void release(bsx_ctx* ctx, DevBuf& b);
-// Records a start event before a kernel launch when profiling is on.
+// Records a start event before a kernel launch when profiling is on and the stream is not being captured.
 void prof_begin(bsx_ctx* ctx);
 // Checks the launch that was just enqueued and counts it.
 bsx_status post_launch(bsx_ctx* ctx, const char* name);

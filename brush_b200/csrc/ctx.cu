@@ -59,6 +59,7 @@ bsx_status ensure(bsx_ctx* ctx, DevBuf& b, size_t bytes) {
     return BSX_OK;
 }
 
+// Under prof_mutex.
 static cudaEvent_t pool_event(bsx_ctx* ctx) {
     if (!ctx->prof_pool.empty()) {
         cudaEvent_t e = ctx->prof_pool.back();
@@ -72,18 +73,31 @@ static cudaEvent_t pool_event(bsx_ctx* ctx) {
 
 void prof_begin_on(bsx_ctx* ctx, cudaStream_t stream) {
     if (!ctx->profiling) return;
-    ctx->prof_start = pool_event(ctx);
-    cudaEventRecord(ctx->prof_start, stream);
+    // an event recorded in a capture belongs to the graph and has no time of its own
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) {
+        cudaGetLastError();
+        return;
+    }
+    if (capture != cudaStreamCaptureStatusNone) return;
+    std::lock_guard<std::mutex> lock(ctx->prof_mutex);
+    cudaEvent_t& start = ctx->prof_start[std::this_thread::get_id()];
+    if (!start) start = pool_event(ctx);  // else that of a call that failed before its launch
+    cudaEventRecord(start, stream);
 }
 void prof_begin(bsx_ctx* ctx) { prof_begin_on(ctx, ctx->stream); }
 
 bsx_status post_launch_on(bsx_ctx* ctx, const char* name, cudaStream_t stream) {
     ctx->launches++;
-    if (ctx->profiling && ctx->prof_start) {
-        cudaEvent_t end = pool_event(ctx);
-        cudaEventRecord(end, stream);
-        ctx->prof_pending.push_back({name, ctx->prof_start, end});
-        ctx->prof_start = nullptr;
+    if (ctx->profiling) {
+        std::lock_guard<std::mutex> lock(ctx->prof_mutex);
+        const auto at = ctx->prof_start.find(std::this_thread::get_id());
+        if (at != ctx->prof_start.end()) {
+            cudaEvent_t end = pool_event(ctx);
+            cudaEventRecord(end, stream);
+            ctx->prof_pending.push_back({name, at->second, end});
+            ctx->prof_start.erase(at);
+        }
     }
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return fail(ctx, BSX_ERR_CUDA, std::string("launch of ") + name + ": " + cudaGetErrorString(e));
@@ -177,6 +191,7 @@ bsx_status bsx_destroy(bsx_ctx* ctx) {
     else cudaDeviceSynchronize();
     if (ctx->d_err) cudaFree(ctx->d_err);
     if (ctx->h_pinned) cudaFreeHost(ctx->h_pinned);
+    for (auto& r : ctx->prof_start) cudaEventDestroy(r.second);
     for (auto& r : ctx->prof_pending) {
         cudaEventDestroy(r.a);
         cudaEventDestroy(r.b);
@@ -233,7 +248,7 @@ const char* bsx_last_error(const bsx_ctx* ctx) {
     return t_error.other.c_str();
 }
 
-uint64_t bsx_launch_count(const bsx_ctx* ctx) { return ctx ? ctx->launches : 0; }
+uint64_t bsx_launch_count(const bsx_ctx* ctx) { return ctx ? ctx->launches.load() : 0; }
 
 bsx_status bsx_profile_enable(bsx_ctx* ctx, int32_t on) {
     if (!ctx) return BSX_ERR_INVALID_ARG;
@@ -246,31 +261,44 @@ bsx_status bsx_profile_collect(bsx_ctx* ctx) {
     cudaSetDevice(ctx->device);
     bsx_status s = check_cuda(ctx, cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
     if (s != BSX_OK) return s;
+    std::lock_guard<std::mutex> lock(ctx->prof_mutex);
     for (auto& r : ctx->prof_pending) {
         float ms = 0.0f;
-        cudaEventSynchronize(r.b);  // launches on other streams
-        cudaEventElapsedTime(&ms, r.a, r.b);
+        // launches on other streams are waited for here
+        cudaError_t e = cudaEventSynchronize(r.b);
+        if (e == cudaSuccess) e = cudaEventElapsedTime(&ms, r.a, r.b);
+        ctx->prof_pool.push_back(r.a);
+        ctx->prof_pool.push_back(r.b);
+        if (e != cudaSuccess) {
+            cudaGetLastError();  // not the next launch's
+            if (s == BSX_OK) s = check_cuda(ctx, e, "launch times");
+            continue;
+        }
         size_t i = 0;
-        while (i < ctx->prof_names.size() && ctx->prof_names[i] != r.name) ++i;
+        while (i < ctx->prof_names.size() && std::strcmp(ctx->prof_names[i], r.name)) ++i;
         if (i == ctx->prof_names.size()) {
-            ctx->prof_names.emplace_back(r.name);
+            ctx->prof_names.push_back(r.name);
             ctx->prof_ms.push_back(0.0);
             ctx->prof_count.push_back(0);
         }
         ctx->prof_ms[i] += ms;
         ctx->prof_count[i] += 1;
-        ctx->prof_pool.push_back(r.a);
-        ctx->prof_pool.push_back(r.b);
     }
     ctx->prof_pending.clear();
-    return BSX_OK;
+    return s;
 }
 
-int32_t bsx_profile_count(const bsx_ctx* ctx) { return ctx ? (int32_t)ctx->prof_names.size() : 0; }
+int32_t bsx_profile_count(const bsx_ctx* ctx) {
+    if (!ctx) return 0;
+    std::lock_guard<std::mutex> lock(ctx->prof_mutex);
+    return (int32_t)ctx->prof_names.size();
+}
 
 bsx_status bsx_profile_entry(const bsx_ctx* ctx, int32_t i, const char** name, double* total_ms, uint64_t* launches) {
-    if (!ctx || i < 0 || i >= (int32_t)ctx->prof_names.size()) return BSX_ERR_INVALID_ARG;
-    if (name) *name = ctx->prof_names[i].c_str();
+    if (!ctx) return BSX_ERR_INVALID_ARG;
+    std::lock_guard<std::mutex> lock(ctx->prof_mutex);
+    if (i < 0 || i >= (int32_t)ctx->prof_names.size()) return BSX_ERR_INVALID_ARG;
+    if (name) *name = ctx->prof_names[i];
     if (total_ms) *total_ms = ctx->prof_ms[i];
     if (launches) *launches = ctx->prof_count[i];
     return BSX_OK;
@@ -279,6 +307,7 @@ bsx_status bsx_profile_entry(const bsx_ctx* ctx, int32_t i, const char** name, d
 bsx_status bsx_profile_reset(bsx_ctx* ctx) {
     if (!ctx) return BSX_ERR_INVALID_ARG;
     bsx_status s = bsx_profile_collect(ctx);
+    std::lock_guard<std::mutex> lock(ctx->prof_mutex);
     ctx->prof_names.clear();
     ctx->prof_ms.clear();
     ctx->prof_count.clear();

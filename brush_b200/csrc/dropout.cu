@@ -166,7 +166,6 @@ bsx_status run(bsx_ctx* ctx, const char* name, const void* x, const void* res, u
                const bsx_dropout_cfg* cfg, void* out, void* stream) {
     if (!ctx || !cfg) return BSX_ERR_INVALID_ARG;
     try {
-        std::lock_guard<std::mutex> lock(ctx->op_mutex);
         DropArgs d;
         if (const char* why = drop_args(cfg, &d)) return fail(ctx, BSX_ERR_INVALID_ARG, why);
         if (cfg->share == 0) return fail(ctx, BSX_ERR_INVALID_ARG, "dropout share must be at least 1");

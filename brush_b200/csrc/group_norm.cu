@@ -132,7 +132,6 @@ bsx_status run(bsx_ctx* ctx, Args a, int32_t dtype, const bsx_group_norm_cfg* cf
                bool bwd, void* stream) {
     if (!ctx || !cfg) return BSX_ERR_INVALID_ARG;
     try {
-        std::lock_guard<std::mutex> lock(ctx->op_mutex);
         auto bad = [&](const char* why) { return fail(ctx, BSX_ERR_INVALID_ARG, why); };
         if (dtype < BSX_F32 || dtype > BSX_F16) return bad("unknown element type");
         if (cfg->param_dtype != BSX_F32 && cfg->param_dtype != dtype)

@@ -187,7 +187,8 @@ BSX_API uint64_t bsx_launch_count(const bsx_ctx* ctx);
 /* Optional per-launch timing with CUDA events on the context's stream.
  * While enabled, every kernel launch is bracketed by two events;
  * bsx_profile_collect synchronises the stream and accumulates the elapsed
- * time per kernel name; entries are read with bsx_profile_entry. */
+ * time per kernel name; entries are read with bsx_profile_entry. Launches
+ * inside stream capture are counted once, when captured, and not timed. */
 BSX_API bsx_status bsx_profile_enable(bsx_ctx* ctx, int32_t on);
 BSX_API bsx_status bsx_profile_collect(bsx_ctx* ctx);
 BSX_API int32_t bsx_profile_count(const bsx_ctx* ctx);
