@@ -67,7 +67,8 @@ class TrainConfig:
     # keep the view-space gradient-norm sum the gradient-threshold densification rule reads
     accumulate_grad2d: bool = False
     # probability that a splat takes no part in a step (regularisation for few views): drawn like
-    # dropout_forward's mask, one draw for a splat, from dropout_seed and the optimizer step's number
+    # dropout_forward's mask, one draw for a splat, from dropout_seed and the optimizer step's number.
+    # AdamScaled's moments and the mean noise act on it as on a splat out of view.
     splat_dropout: float = 0.0
     dropout_seed: int = 42
 
@@ -131,6 +132,23 @@ class RefineConfig:
         """The training loop's gate (crates/brush-process/src/train_stream.rs:481-483)."""
         progress = min(max(np.float32(phase_iter) / np.float32(max(phase_total, 1)), 0.0), 1.0)
         return phase_iter > 0 and phase_iter % self.refine_every == 0 and progress <= 0.95
+
+
+def check_splat_dropout(p: float) -> None:
+    """Refuses what ``bsx_trainer_set_dropout`` refuses, for every exchange alike."""
+    if not 0.0 <= float(p) < 1.0:
+        raise _lib.BsxError(1, f"splat dropout must lie in [0, 1), got {p}")
+
+
+def step_opacities(raw_opacities: torch.Tensor, config: TrainConfig, step: int) -> torch.Tensor:
+    """The opacity logits that step ``step`` renders: -inf, which is culled and has no gradient, where
+    splat dropout leaves a splat out (the native step's mask)."""
+    check_splat_dropout(config.splat_dropout)
+    if config.splat_dropout == 0.0:
+        return raw_opacities
+    drop = DropoutConfig(p=config.splat_dropout, seed=int(config.dropout_seed) % 2**64, step=step)
+    kept = dropout_forward(torch.ones_like(raw_opacities), drop) > 0
+    return torch.where(kept, raw_opacities, float("-inf"))
 
 
 def _world_of(process_group) -> int:
@@ -230,6 +248,7 @@ class _NativeTrainer:
 class SplatTrainer:
     def __init__(self, config: TrainConfig, splats: Splats, process_group=None, gather_stats: bool = True,
                  shard_optimizer: bool = True, exchange: str = "auto", keep_gradients: bool = False):
+        check_splat_dropout(config.splat_dropout)
         self.config = config
         # The single-GPU step applies AdamScaled inside the projection backward;
         # keep_gradients also writes the dense gradients to ``grads``.
@@ -379,10 +398,7 @@ class SplatTrainer:
     def _nccl_step(self, camera, img_size, gt_packed, splats, compute_refine_weight) -> TrainStepStats:
         self.step_count += 1
         cfg = self.config
-        opac = splats.raw_opacities
-        if cfg.splat_dropout > 0.0:  # a logit that is not finite is culled, and has no gradient
-            drop = DropoutConfig(p=cfg.splat_dropout, seed=cfg.dropout_seed, step=self.step_count)
-            opac = torch.where(dropout_forward(torch.ones_like(opac), drop) > 0, opac, float("-inf"))
+        opac = step_opacities(splats.raw_opacities, cfg, self.step_count)
         out = render(camera, img_size, splats.transforms, splats.sh_coeffs, opac,
                      splats.render_mode, cfg.background_color, _lib.PASS_BACKWARD)
         ssim_w = cfg.ssim_weight

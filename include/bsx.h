@@ -435,7 +435,8 @@ BSX_API bsx_status bsx_trainer_grad_buffers(bsx_trainer* tr, float** d_v_transfo
                                             float** d_v_raw_opac, float** d_v_refine_weight);
 /* Splat dropout (no counterpart in the reference; off by default): in each following training step a
  * splat takes no part with probability p, in [0, 1): it is not rendered, has no gradient and does not
- * count as visible. Splat i takes draw i of bsx_dropout_cfg's mask for (p, seed, step), step being the
+ * count as visible; the optimizer's moments and the mean noise act on it as on a splat out of view.
+ * Splat i takes draw i of bsx_dropout_cfg's mask for (p, seed, step), step being the
  * number of the optimizer step, from 1; opacities are not rescaled. Ranks with the same seed leave
  * the same splats out. */
 BSX_API bsx_status bsx_trainer_set_dropout(bsx_trainer* tr, double p, uint64_t seed);
