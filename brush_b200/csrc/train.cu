@@ -594,16 +594,16 @@ bsx_status bsx_train_step_dp(bsx_trainer* tr, const bsx_camera* cam, uint32_t w,
         gp.world = world;
         gp.rank = rank;
     }
-    bsx_render_out out{};
-    bsx_status s = forward_backward(tr, cam, w, h, gt, sp->d_transforms[rank], sp->d_sh_coeffs[rank],
-                                    sp->d_raw_opac[rank], sp->d_v_transforms[rank], sp->d_v_sh_coeffs[rank],
-                                    sp->d_v_raw_opac[rank], ex->d_refine[rank], refine, d_loss, tr->step + 1, &out, nullptr,
-                                    push ? &gp : nullptr);
-    if (s != BSX_OK) return s;
+    // The moments first: where they start anew, so does the step's number, which splat dropout draws by.
     const uint32_t rb = (uint32_t)((uint64_t)tr->n * rank / world), re = (uint32_t)((uint64_t)tr->n * (rank + 1) / world);
     float* m[3];
     float* v[3];
-    s = ensure_moments(tr, re - rb, world, rank, m, v);
+    bsx_status s = ensure_moments(tr, re - rb, world, rank, m, v);
+    if (s != BSX_OK) return s;
+    bsx_render_out out{};
+    s = forward_backward(tr, cam, w, h, gt, sp->d_transforms[rank], sp->d_sh_coeffs[rank], sp->d_raw_opac[rank],
+                         sp->d_v_transforms[rank], sp->d_v_sh_coeffs[rank], sp->d_v_raw_opac[rank], ex->d_refine[rank],
+                         refine, d_loss, tr->step + 1, &out, nullptr, push ? &gp : nullptr);
     if (s != BSX_OK) return s;
     const Rates r = next_rates(tr);
     tr->step++;

@@ -118,3 +118,50 @@ def test_collective_step_refuses_what_the_native_one_refuses(cuda, monkeypatch):
         tr.config.splat_dropout = p
         with pytest.raises(bsx.BsxError):
             tr.step(cam, SIZE, gt, g)
+
+
+def _exchange(g):
+    """The structures of bsx_train_step_dp for one rank, over the splats' own tensors."""
+    from brush_b200 import _lib
+
+    n, c = g.num_splats, g.sh_coeffs_per_splat
+    z = lambda *shape, **kw: torch.zeros(shape, device="cuda", **kw)  # noqa: E731
+    bufs = dict(flags=z(_lib.BSX_DP_FLAG_WORDS, dtype=torch.int32), refine=z(n), gate=z(n), vt=z(n, 10), vs=z(n, c, 3), vo=z(n))
+    ex, sp = _lib.DpExchange(), _lib.DpSplats()
+    ex.rank, ex.world, ex.refine_rows, ex.timeout_ns = 0, 1, n, int(1e9)
+    for field, t in ((ex.d_flags, bufs["flags"]), (ex.d_refine, bufs["refine"]), (ex.d_gate, bufs["gate"]),
+                     (sp.d_transforms, g.transforms), (sp.d_sh_coeffs, g.sh_coeffs), (sp.d_raw_opac, g.raw_opacities),
+                     (sp.d_v_transforms, bufs["vt"]), (sp.d_v_sh_coeffs, bufs["vs"]), (sp.d_v_raw_opac, bufs["vo"])):
+        field[0] = t.data_ptr()
+    return ex, sp, bufs
+
+
+def test_data_parallel_step_counts_its_mask_from_the_moments(cuda, bsx_lib):
+    """bsx_train_step_dp draws the mask of the step that it reports, also where the moments start anew."""
+    import brush_b200 as bsx
+
+    g, cam, gt = _scene()
+    n, L = g.num_splats, bsx_lib.lib()
+    tr = bsx.SplatTrainer(_config(), g)
+    ex, sp, bufs = _exchange(g)
+
+    def step():
+        st, cc = bsx_lib.TrainStats(), cam.to_c()
+        masks = [_visible(g, cam, ref.mask(n, P, SEED, k)) for k in (1, 2, 3, 4)]
+        assert len({c for c, _ in masks}) == 4  # each mask sees another number of splats
+        tr.native.ctx.check(L.bsx_train_step_dp(tr.native.handle, C.byref(cc), *SIZE, gt.data_ptr(), C.byref(ex), C.byref(sp),
+                                                1, tr.loss.data_ptr(), C.byref(st)))
+        torch.cuda.synchronize()
+        return st.step, [c for c, _ in masks].index(st.num_visible) + 1
+
+    assert step() == (1, 1)
+    assert step() == (2, 2)
+    # another shard's moments: the next step of all splats starts from zero, as the single-GPU step's does
+    half = [t[:n // 2].clone() for s in tr.native.optimizer_state() for t in s]
+    tr.native.load_optimizer_state(half[:3], half[3:], n // 2, 2, 0)
+    assert step() == (1, 1)
+    assert step() == (2, 2)
+    tr.native.load_optimizer_state(half[:3], half[3:], n // 2, 2, 0)
+    st = tr.step(cam, SIZE, gt, g)
+    assert tr.step_count == 1
+    tr.close()
