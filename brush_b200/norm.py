@@ -35,6 +35,8 @@ def _sizes(shape: torch.Size, dtype: torch.dtype, param: torch.dtype, groups: in
     n, pixels, c = shape[0], math.prod(shape[1:-1]), shape[-1]
     if groups < 1 or c < 1 or c % groups:
         raise ValueError(f"{c} channels cannot be split into {groups} groups")
+    if c >= 1 << 32:  # the C interface would see its low half
+        raise ValueError("samples x channels must stay below 2^31")
     if pixels == 0:
         raise ValueError("a sample must have at least one pixel")
     if not eps >= 0.0:
