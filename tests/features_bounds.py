@@ -15,6 +15,10 @@ U = ref.U
 CHAIN = 640
 
 
+def normal(shape, seed, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
 def _parts(z, act):
     """w, w', w'' of the gate s(w(z))."""
     if act == "silu":
