@@ -93,9 +93,10 @@ __device__ __forceinline__ void single8(const T* __restrict__ x, const T* __rest
 
 // One thread per block of eight elements, U blocks a thread, kThreads apart. Memory bounds it: a million rows of 48
 // floats, a draw a row, 384 MB in 60.6 us (6.3 TB/s, 97 % of the measured copy rate); 33 M bf16 elements with a
-// residual, 199 MB in 32.3 us (94 %). Without a residual 16-bit elements come near the issue limit (seven rounds, the
-// comparisons and conversions are about 13 instructions an element): 29 M f16 elements, 58 MB, 12.7 us (69 %, of
-// which launch and the last wave of blocks take about 3 us). Tried: a grid of resident blocks that loops (13.7 to
+// residual, 199 MB in 32.3 us (94 %). Without a residual 16-bit elements have 14 instructions each (seven rounds, the
+// comparisons and conversions): 14.4 M f16 elements, 58 MB, 12.7 us (69 %). Neither memory nor issue bounds that: while
+// an SM has blocks it issues 63 % of the time, but over the whole launch 47 %, since three waves of blocks begin with
+// loads and end unevenly. Tried: a grid of resident blocks that loops (13.7 to
 // 14.9 us there, 75 us for the rows): the loads of an iteration then wait for the iteration before.
 template <class T, bool RES, bool ROWS, bool VEC, int U>
 __global__ void __launch_bounds__(kThreads, 4)

@@ -89,23 +89,22 @@ __device__ __forceinline__ bool keep1(const DropArgs& d, uint32_t step, uint64_t
     return ((j & 4 ? e : c) >> (j & 1 ? 16 : 0) & 0xffffu) >= d.t_lo;
 }
 
-// v[j] = draw 8 q + FIRST + j kept ? v[j] scale : 0. Without a tie a draw is decided by one comparison on the
+// v[j] = draw 8 q + j kept ? v[j] scale : 0. Without a tie a draw is decided by one comparison on the
 // whole word (odd draws) or on the word shifted up (even ones).
-template <int V, int FIRST = 0>
+template <int V>
 __device__ __forceinline__ void drop_values(const DropArgs& d, uint32_t step, uint64_t q, float (&v)[V]) {
     const uint32_t q0 = (uint32_t)q, q1 = (uint32_t)(q >> 32);
     const uint4 w = philox7(d, q0, q1, step, 0u);
     if (any_tie(d, w)) {
         const uint32_t keep = tie_bits(d, step, q0, q1, w);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = keep >> (FIRST + j) & 1u ? v[j] * d.scale : 0.0f;
+        for (int j = 0; j < V; ++j) v[j] = keep >> j & 1u ? v[j] * d.scale : 0.0f;
     } else {
         const uint32_t top = d.t_hi << 16 | 0xffffu;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int k = FIRST + j;
-            const uint32_t word = k < 2 ? w.x : k < 4 ? w.y : k < 6 ? w.z : w.w;
-            v[j] = (k & 1 ? word : word << 16) > top ? v[j] * d.scale : 0.0f;
+            const uint32_t word = j < 2 ? w.x : j < 4 ? w.y : j < 6 ? w.z : w.w;
+            v[j] = (j & 1 ? word : word << 16) > top ? v[j] * d.scale : 0.0f;
         }
     }
 }

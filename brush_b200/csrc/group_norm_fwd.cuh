@@ -124,11 +124,12 @@ __global__ void __launch_bounds__(kThreads, 2) small_fwd_kernel(const Plan p, co
 // Large samples: one cooperative launch. Every thread copies its vectors of the block's coming batches of rows into
 // its own places of a ring in shared memory, some batches ahead. First pass: mean and sum of squared deviations of
 // each group in each segment, to the workspace. Deviations are taken from a pivot, the group's mean over the block's
-// first batch, so that no large mean cancels (what the pivot is off by enters the sum of squares at most a quarter of
-// the block's rows times over). Grid barrier. Second pass, last row first: the segments' statistics are joined, and the rows are
+// first batch, so that no large mean cancels (what the pivot is off by enters the sum of squares at most a batch's
+// share of the block's rows times over). Grid barrier. Second pass, last row first: the segments' statistics are joined, and the rows are
 // normalised out of the ring, which still holds the last ones; the others come again.
-// A full frame of 64 bf16 channels (265 MB, larger than L2) takes 139 us: 27 MB stay in the rings, so 765 MB cross
-// DRAM, 5.5 TB/s, 84 % of the measured copy rate; read once and written once it would be 81 us. Keeping more in L2
+// A full frame of 64 bf16 channels (265 MB, larger than L2) takes 136 us: 27 MB stay in the rings, so 482 MB are read
+// from DRAM (measured; some 20 MB hit L2) and 265 MB written (213 of them before the kernel ends, the others are in L2
+// then): 5.5 TB/s, 84 % of the measured copy rate; read once and written once it would be 81 us. Keeping more in L2
 // (evict_last, prefetches between the passes) gave 3 % at most; deeper rings, bulk copies and other batch sizes
 // nothing. 8 x 64 x 64 x 256 (17 MB, all of it stays) takes 15.5 us against 5.1: 5 us until the last row has arrived,
 // 1 for the sums, 1.5 each for the barrier and the join, 4 for the second pass, which the special-function unit

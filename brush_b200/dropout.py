@@ -5,6 +5,9 @@ and counted by (element, step), as the mean noise of the training step does, so 
 draws it again instead of reading it, runs are reproducible and ranks with the same seed agree.
 ``share`` elements in a row use one draw: ``share=1`` drops elements, ``share=C`` drops whole
 rows of a ``[N, C]`` tensor (splats, or the rows of a residual branch).
+
+Forward and backward are calls of their own, as everywhere in this package: autograd does not record
+them, and a result never requires a gradient (wrap the two in a ``torch.autograd.Function`` for that).
 """
 from __future__ import annotations
 

@@ -2,6 +2,8 @@
 layout of the renders (a permuted view of a ``channels_last`` tensor is one without a copy).
 
 Statistics, gates and sums are formed in 32 bits whatever the tensor's type, and rounded once.
+Autograd does not record the calls: a result never requires a gradient, and the backward takes the
+forward's inputs, statistics and configuration.
 """
 from __future__ import annotations
 

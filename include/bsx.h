@@ -585,8 +585,8 @@ BSX_API bsx_status bsx_mean_noise_step(bsx_ctx* ctx, float* d_transforms, const 
  * No counterpart in the reference. They serve training next to the renderer: splats or
  * features dropped at random (beside the mean noise above), and learned networks on
  * channels-last images such as the renders. Unlike the calls above they take their stream
- * as an argument, keep nothing in the context but its error text, launch count and launch
- * times, and need no memory beyond what the caller passes: calls on several streams, from
+ * as an argument, keep nothing in the context but its error texts, launch count and launch
+ * times (which are safe between threads), and need no memory beyond what the caller passes: calls on several streams, from
  * several threads and inside stream capture may overlap. Tensors are contiguous, need no
  * alignment beyond their element's (16 bytes is faster), and their element type is one
  * of bsx_dtype; sums, statistics and products are formed in 32 bits and rounded once. */
@@ -627,6 +627,8 @@ typedef enum bsx_activation {
 /* Group norm of x [N, pixels, C], channels last: for sample n and group g of C / groups
  * channels, mean and biased variance over the group's pixels and channels, rstd =
  * 1 / sqrt(var + eps), z = weight[c] (x - mean) rstd + bias[c], out = dropout(act(z)).
+ * Squares of (x - mean) must stay finite in 32 bits. Far below zero the activations and their
+ * slopes are 0: a channel is switched off by any bias 50 and more below its other values, down to the type's lowest.
  * weight and bias may be null (1 and 0) and have type param_dtype (x's type or BSX_F32);
  * dropout may be null, its share must be 1, and it draws the mask that bsx_dropout_fwd
  * draws for the same output tensor. mean and rstd [N, groups] are float. */
