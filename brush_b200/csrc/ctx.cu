@@ -75,12 +75,17 @@ void prof_begin_on(bsx_ctx* ctx, cudaStream_t stream) {
     if (!ctx->profiling) return;
     // an event recorded in a capture belongs to the graph and has no time of its own
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) {
-        cudaGetLastError();
+    const cudaError_t e = cudaStreamIsCapturing(stream, &capture);
+    if (e != cudaSuccess) cudaGetLastError();
+    std::lock_guard<std::mutex> lock(ctx->prof_mutex);
+    if (e != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+        const auto left = ctx->prof_start.find(std::this_thread::get_id());
+        if (left != ctx->prof_start.end()) {
+            ctx->prof_pool.push_back(left->second);
+            ctx->prof_start.erase(left);
+        }
         return;
     }
-    if (capture != cudaStreamCaptureStatusNone) return;
-    std::lock_guard<std::mutex> lock(ctx->prof_mutex);
     cudaEvent_t& start = ctx->prof_start[std::this_thread::get_id()];
     if (!start) start = pool_event(ctx);  // else that of a call that failed before its launch
     cudaEventRecord(start, stream);
