@@ -207,7 +207,7 @@ __device__ __forceinline__ float rcp_fast(float x) {
 // 2^-63, must not be multiplied by a far z, nor by the slope's terms, which grow with it: 2^-62 is
 // taken off every s and the result clamped to [0, 1], both in the multiplication that forms it. s is
 // off by a few units in the last place, by |w| of them (the rounding of w log2 e) and by 2^-62, and
-// is 0 from w = -43.7 down.
+// is 0 from w = -43 down.
 constexpr float kLog2e = 1.4426950408889634f, kGelu1 = 1.5957691216057308f, kGelu3 = 0.044715f;
 constexpr float kMostExponent = 63.0f, kLeft = 2.168404344971009e-19f;  // 2^-62
 template <int V>

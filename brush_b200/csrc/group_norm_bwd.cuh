@@ -262,8 +262,9 @@ __global__ void __launch_bounds__(kThreads) small_bwd_kernel(const Plan p, const
 // the channels are dealt to the warps of the grid.
 // A half-resolution frame of 128 bf16 channels (133 MB each of x, v and v_x) takes 110 us: 27 MB stay in the rings,
 // 468 MB are read from DRAM (measured; some 36 MB hit L2) and 133 MB written (83 before the kernel ends), 5.5 TB/s, 84 %
-// of the measured copy rate; read and written once it would be 61 us. 8 x 64 x 64 x 256 takes 23 us against 7.7: 9 us for the first pass (34 MB, with two special-function uses and about 90 FP32
-// operations a vector lane), 5 for sums, barrier and join, 6 for the second pass, 1 to 2 for the channels.
+// of the measured copy rate; read and written once it would be 61 us. 8 x 64 x 64 x 256 takes 23 us against 7.7: 9 us
+// for the first pass (34 MB, with two special-function uses and about 90 FP32 operations a vector lane), 5 for sums,
+// barrier and join, 6 for the second pass, 1 to 2 for the channels.
 template <class T, int V, int L, int ACT, int DROP, bool S>
 __global__ void __launch_bounds__(kThreads, 1) large_bwd_kernel(const Plan p, const Args a) {
     extern __shared__ float smem[];
