@@ -67,3 +67,33 @@ def test_group_norm_channel_off_leaves_the_others(cuda, act, dtype):
         got = bsx.group_norm_backward(v, x, w, b, mean, rstd, cfg)
         want = bsx.group_norm_backward(zero, x, w, b, mean, rstd, cfg)
         assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("n,sp,c,g", [(2, (9, 7), 64, 16), (1, (200, 150), 64, 16), (2, (40_001,), 37, 37), (3, (13, 7), 21, 7)],
+                         ids=["small", "large", "odd", "single"])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_group_norm_nan_parameters_stay_in_their_channels(cuda, act, n, sp, c, g, dtype):
+    """Lanes share reciprocals: a NaN among the weights or biases reaches its own channel, and the gradients of its group."""
+    import brush_b200 as bsx
+
+    x, v = _normal((n, *sp, c), 7, dtype).cuda(), _normal((n, *sp, c), 8, dtype).cuda()
+    per, cfg = c // g, bsx.GroupNormConfig(groups=g, activation=act)
+    for which in (0, 1):
+        params = [torch.ones(c), torch.zeros(c)]
+        params[which][5] = float("nan")
+        w, b = (t.cuda() for t in params)
+        out, mean, rstd = bsx.group_norm_forward(x, w, b, cfg)
+        v_x, v_w, v_b = bsx.group_norm_backward(v, x, w, b, mean, rstd, cfg)
+        channel = torch.arange(c, device="cuda") == 5
+        group = torch.arange(c, device="cuda") // per == 5 // per
+        assert mean.isfinite().all() and rstd.isfinite().all()
+        assert torch.equal(out.isnan(), channel.expand_as(out)) and out[..., ~channel].isfinite().all()
+        if act == "none" and which == 1:  # the bias has no part in the gradients
+            assert all(t.isfinite().all() for t in (v_x, v_w, v_b))
+            continue
+        assert torch.equal(v_x.isnan(), group.expand_as(v_x)) and v_x[..., ~group].isfinite().all()
+        if act == "none":  # nor has the weight in its own
+            assert v_w.isfinite().all() and v_b.isfinite().all()
+        else:
+            assert torch.equal(v_w.isnan(), channel) and torch.equal(v_b.isnan(), channel)
